@@ -428,6 +428,112 @@ int shady_qkv_proj_append(shady_ctx *ctx, const shady_append_params *p, const sh
                           const uint32_t *d_pos_start, const uint32_t *d_pos_h, const uint32_t *d_pos_w);
 
 /* ===================================================================================== */
+/* Row-scaled 8-bit KV cache (no reference counterpart: the reference's cache is f32,      */
+/* model.rs:241-256)                                                                       */
+/* ===================================================================================== */
+/* The per-cache scales of SHADY_F8E4M3 / SHADY_F8E5M2 have to be known before the first row is written; here every
+ * (row, kv head) carries a scale of its own, computed as the row is written:
+ *     scale = clamp(max|x| / 127, 2^-60, 2^60)        code = clamp(round-to-nearest-even(x / scale), -127, 127)
+ * and an element is code * scale.  Codes are stored as one byte, code + 128.  A NaN element is stored as 0 and does
+ * not count in max|x|; an infinity makes the scale 2^60 and is stored as +-127 of it.
+ * Row r of sequence s is row  s * seq_rows + r  of  codes [rows][num_kv_heads][head_dim] u8  and
+ * scales [rows][num_kv_heads] f32  (K and V each have both), or, with d_page_table set, row r % page_rows of page
+ * d_page_table[s * max_pages_per_seq + r / page_rows] of pools [page][page_rows][...]; page_rows is a multiple of 16.
+ * With num_pages set, table entries of num_pages or more are not followed: nothing is stored to such a page and its
+ * rows read as zero.  head_dim is 64, 128 or 256; code arrays are 16-byte aligned.  Zero the struct before filling it. */
+typedef struct {
+    void *d_k_codes;
+    void *d_v_codes;
+    float *d_k_scales;
+    float *d_v_scales;
+    uint64_t seq_rows;              /* rows between consecutive sequences (one allocation); not read with a page table */
+    const uint32_t *d_page_table;   /* device [num_seqs][max_pages_per_seq], or NULL */
+    uint32_t page_rows;
+    uint32_t max_pages_per_seq;
+    uint32_t num_pages;             /* pages of the pools; 0 = table entries are not checked */
+    uint32_t _pad;
+} shady_rowq_cache;
+
+/* shady_kv_append_rope (same parameters and arithmetic up to the store) into a row-scaled cache.  Beside the cache,
+ * d_k_out / d_v_out (both or neither) receive the rows as the cache now holds them, code * scale rounded to q_dtype,
+ * packed [tokens][num_kv_heads][head_dim]: what the attention of the same step reads (shady_attn_prefill_rule), so
+ * that a prompt attends to the values that its later decode steps will see.  p->in_dtype and p->q_dtype are f32, f16 or bf16.
+ * p->write_k_back is not supported and must be 0.  d_tok_start: NULL for num_seqs * tokens_per_seq tokens, token
+ * (s, j) in row s * tokens_per_seq + j; else device [num_seqs + 1], the first packed token of every sequence (not
+ * falling; a sequence may have none), of which total_tokens is an upper bound known to the host: rows of the outputs
+ * at or behind d_tok_start[num_seqs] are left as they were.  A position at or behind the end of a sequence's cache
+ * (seq_rows, or max_pages_per_seq pages) stores nothing in the cache; its outputs are written all the same. */
+int shady_kv_append_rowq(shady_ctx *ctx, const shady_append_params *p, const void *d_q_proj_full, const void *d_k_proj,
+                         const void *d_v_proj, void *d_q_out, float *d_q_gate, void *d_k_out, void *d_v_out,
+                         const shady_rowq_cache *cache, const uint16_t *d_qk_norm_bf16, const uint32_t *d_pos_start,
+                         const uint32_t *d_pos_h, const uint32_t *d_pos_w, const uint32_t *d_tok_start,
+                         uint32_t total_tokens);
+
+/* Reads row ranges of a row-scaled cache back: rows [d_row_start[s], d_row_start[s] + n_s) of sequence s, with
+ * n_s = d_out_start[s + 1] - d_out_start[s] (device [num_seqs + 1], not falling), go to rows d_out_start[s].. of
+ * d_k_out / d_v_out [total_rows][num_kv_heads][head_dim] in out_dtype (f32, f16 or bf16; code * scale, rounded once).
+ * Either output may be NULL.  total_rows is an upper bound of d_out_start[num_seqs] known to the host; output rows
+ * behind it are left as they were.  d_row_start NULL = 0 for every sequence.  Cache rows behind the end of a
+ * sequence's cache read as zero. */
+int shady_kv_read_rowq(shady_ctx *ctx, const shady_rowq_cache *cache, uint32_t num_kv_heads, uint32_t head_dim,
+                       uint32_t num_seqs, const uint32_t *d_row_start, const uint32_t *d_out_start, uint32_t total_rows,
+                       void *d_k_out, void *d_v_out, uint32_t out_dtype);
+
+/* ===================================================================================== */
+/* Attention under a score rule (no reference counterpart: the reference scales by          */
+/* 1/sqrt(head_dim) and masks causally, gqa_attention_head.wgsl:63-94)                      */
+/* ===================================================================================== */
+/* For a query at position i of sequence s (its row in the cache) and the cache row j, head h:
+ *     z = q.k * scale;   z = cap * tanh(z / cap) if cap > 0;   z = z - d_slopes[h] * |i - j| if d_slopes
+ * and row j is seen iff  j < rows of the sequence,  j >= the query's first visible row (d_doc_start), and
+ *     j < d_prefix_lens[s]  or  ( j <= i  and  ( window == 0  or  i - j < window ) ).
+ * So prefix rows are seen by every query of the sequence, before and after them, also behind a window; packed
+ * documents are kept apart by the first row of each token's document.  A query that sees no row yields zeros and
+ * lse = -inf.  Rows that a query does not see have no influence on it if they hold finite values; rows at or behind
+ * the end of a sequence have none whatever they hold. */
+typedef struct {
+    float scale;                    /* 0 = 1/sqrt(head_dim); else > 0 */
+    float cap;                      /* 0 = no cap; else > 0 */
+    uint32_t window;                /* 0 = no window */
+    uint32_t _pad;
+    const float *d_slopes;          /* device [num_q_heads] (any sign, finite), or NULL */
+    const uint32_t *d_prefix_lens;  /* device [num_seqs], or NULL */
+    const uint32_t *d_doc_start;    /* decode: device [num_seqs]; prefill: device [tokens], packed; or NULL */
+} shady_score_rule;
+
+/* Attention of one new token per sequence, at position d_seq_lens[s] - 1, over the d_seq_lens[s] rows of its cache (a
+ * length of 0 yields zeros and lse = -inf).  Exactly one of `cache` (f16 / bf16; base + seq_stride, pointer arrays or
+ * paged) and `rowq` is given.  p->head_dim is 64, 128 or 256, p->num_splits 0; p->q_dtype is SHADY_F32, the cache
+ * dtype, or for a row-scaled cache any of f32, f16 and bf16 (Q is rounded to the cache dtype, f16 for a row-scaled
+ * cache after a power of two per head has been taken out); p->out_dtype any of the three.  d_lse: optional
+ * [num_seqs][nh] f32, natural logarithm of sum exp(z).  Lengths are read on the device only, so a captured launch
+ * serves growing sequences.  Rows are cut into equal shares of one resident grid and joined by the CTA that finishes a
+ * (sequence, kv head) last, in the order of the shares: results do not depend on which CTA that was.  d_workspace: at
+ * least shady_decode_rule_workspace_size bytes, 16-byte aligned, shady_decode_rule_workspace_init once before its
+ * first use; every call leaves it ready for the next.  Calls that share a workspace must not overlap on the GPU. */
+int shady_decode_rule_workspace_size(shady_ctx *ctx, const shady_decode_params *p, size_t *bytes);
+int shady_decode_rule_workspace_init(shady_ctx *ctx, const shady_decode_params *p, void *d_workspace, size_t workspace_bytes);
+int shady_attn_decode_rule(shady_ctx *ctx, const shady_decode_params *p, const shady_score_rule *rule, const void *d_q,
+                           const shady_kv_cache *cache, const shady_rowq_cache *rowq, const uint32_t *d_seq_lens,
+                           void *d_out, float *d_lse, void *d_workspace, size_t workspace_bytes);
+
+/* Attention of many tokens per sequence over rows that are in the cache already, the tokens' own rows among them:
+ * whole prompts, or a chunk of a prompt behind earlier rows.  Sequence s has the packed tokens d_q_starts[s] ..
+ * d_q_starts[s + 1] - 1 (device [num_seqs + 1], not falling) and d_kv_lens[s] rows (device); its t-th token is at
+ * position d_kv_lens[s] - tokens + t.  A sequence may have no tokens; one with more tokens than rows is computed for
+ * its last d_kv_lens[s] tokens, the others are treated as seeing no row.  d_q, d_out [total_q][nh][hd] in p->dtype,
+ * d_lse optional [total_q][nh] f32; total_q is an upper bound of d_q_starts[num_seqs] known to the host, and output
+ * rows behind it are left as they were.  Cache (16-bit, p->dtype): d_k_base / d_v_base hold cache_rows rows
+ * [cache_rows][num_kv_heads][head_dim]; sequence s starts at row d_kv_starts[s] (packed rows), or with d_kv_starts NULL
+ * at s * seq_stride / (num_kv_heads * head_dim), or rows come through the page table (page_rows any multiple of
+ * 16; the pools hold cache_rows / page_rows pages, and rows of a page beyond them read as zero).  p->head_dim 128 or 256, at most 128 query heads per
+ * kv head, p->seq_len is not read.  Everything is read on the device: no workspace, capturable. */
+int shady_attn_prefill_rule(shady_ctx *ctx, const shady_prefill_params *p, const shady_score_rule *rule, const void *d_q,
+                            const shady_kv_cache *cache, uint64_t cache_rows, const uint32_t *d_q_starts,
+                            uint32_t total_q, const uint32_t *d_kv_starts, const uint32_t *d_kv_lens, void *d_out,
+                            float *d_lse);
+
+/* ===================================================================================== */
 /* Synthetic data — counter-based N(0,1) fill used by the benchmark and the tests         */
 /* (no reference counterpart: the reference has no benchmark inputs).                     */
 /* ===================================================================================== */

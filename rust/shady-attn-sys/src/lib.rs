@@ -110,6 +110,35 @@ pub struct ShadyGptqWeight {
     pub _pad: u32,
 }
 
+/// `shady_rowq_cache` — same fields, same order.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct ShadyRowqCache {
+    pub d_k_codes: *mut c_void,
+    pub d_v_codes: *mut c_void,
+    pub d_k_scales: *mut f32,
+    pub d_v_scales: *mut f32,
+    pub seq_rows: u64,
+    pub d_page_table: *const u32,
+    pub page_rows: u32,
+    pub max_pages_per_seq: u32,
+    pub num_pages: u32,
+    pub _pad: u32,
+}
+
+/// `shady_score_rule` — same fields, same order.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct ShadyScoreRule {
+    pub scale: f32,
+    pub cap: f32,
+    pub window: u32,
+    pub _pad: u32,
+    pub d_slopes: *const f32,
+    pub d_prefix_lens: *const u32,
+    pub d_doc_start: *const u32,
+}
+
 extern "C" {
     pub fn shady_ctx_create(device: c_int, stream: *mut c_void, out: *mut *mut ShadyCtx) -> c_int;
     pub fn shady_ctx_destroy(ctx: *mut ShadyCtx) -> c_int;
@@ -149,5 +178,11 @@ extern "C" {
     pub fn shady_sigmoid_mul(ctx: *mut ShadyCtx, d_x: *mut f32, d_gate: *const f32, n: u32) -> c_int;
     pub fn shady_gptq_matvec(ctx: *mut ShadyCtx, w: *const ShadyGptqWeight, d_x: *const f32, d_y: *mut f32, num_vecs: u32) -> c_int;
     pub fn shady_qkv_proj_append(ctx: *mut ShadyCtx, p: *const ShadyAppendParams, wq: *const ShadyGptqWeight, wk: *const ShadyGptqWeight, wv: *const ShadyGptqWeight, d_x: *const f32, d_q_out: *mut c_void, d_q_gate: *mut f32, cache: *const ShadyKvCache, d_qk_norm_bf16: *const u16, d_pos_start: *const u32, d_pos_h: *const u32, d_pos_w: *const u32) -> c_int;
+    pub fn shady_kv_append_rowq(ctx: *mut ShadyCtx, p: *const ShadyAppendParams, d_q_proj_full: *const c_void, d_k_proj: *const c_void, d_v_proj: *const c_void, d_q_out: *mut c_void, d_q_gate: *mut f32, d_k_out: *mut c_void, d_v_out: *mut c_void, cache: *const ShadyRowqCache, d_qk_norm_bf16: *const u16, d_pos_start: *const u32, d_pos_h: *const u32, d_pos_w: *const u32, d_tok_start: *const u32, total_tokens: u32) -> c_int;
+    pub fn shady_kv_read_rowq(ctx: *mut ShadyCtx, cache: *const ShadyRowqCache, num_kv_heads: u32, head_dim: u32, num_seqs: u32, d_row_start: *const u32, d_out_start: *const u32, total_rows: u32, d_k_out: *mut c_void, d_v_out: *mut c_void, out_dtype: u32) -> c_int;
+    pub fn shady_decode_rule_workspace_size(ctx: *mut ShadyCtx, p: *const ShadyDecodeParams, bytes: *mut usize) -> c_int;
+    pub fn shady_decode_rule_workspace_init(ctx: *mut ShadyCtx, p: *const ShadyDecodeParams, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn shady_attn_decode_rule(ctx: *mut ShadyCtx, p: *const ShadyDecodeParams, rule: *const ShadyScoreRule, d_q: *const c_void, cache: *const ShadyKvCache, rowq: *const ShadyRowqCache, d_seq_lens: *const u32, d_out: *mut c_void, d_lse: *mut f32, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn shady_attn_prefill_rule(ctx: *mut ShadyCtx, p: *const ShadyPrefillParams, rule: *const ShadyScoreRule, d_q: *const c_void, cache: *const ShadyKvCache, cache_rows: u64, d_q_starts: *const u32, total_q: u32, d_kv_starts: *const u32, d_kv_lens: *const u32, d_out: *mut c_void, d_lse: *mut f32) -> c_int;
     pub fn shady_fill_randn(ctx: *mut ShadyCtx, d_dst: *mut c_void, n: u64, dtype: u32, seed: u64, tensor_id: u64, first_idx: u64) -> c_int;
 }

@@ -25,6 +25,8 @@ EXPORTS = [
     "shady_prefill_workspace_size", "shady_attn_prefill_append",
     "shady_prefill_ragged_workspace_size", "shady_attn_prefill_ragged", "shady_attn_prefill_append_ragged",
     "shady_gptq_matvec", "shady_qkv_proj_append",
+    "shady_kv_append_rowq", "shady_kv_read_rowq", "shady_decode_rule_workspace_size", "shady_decode_rule_workspace_init",
+    "shady_attn_decode_rule", "shady_attn_prefill_rule",
     "shady_sigmoid_mul", "shady_fill_randn", "shady_ipc_export", "shady_ipc_open", "shady_ipc_close",
     "shady_combine_p2p_buffer_size", "shady_attn_combine_p2p", "shady_attn_decode_shard_p2p",
 ]
@@ -70,6 +72,17 @@ class PrefillParams(C.Structure):
 
 class PrefillBatch(C.Structure):
     _fields_ = [("h_seq_lens", C.c_void_p), ("h_k_ptrs", C.c_void_p), ("h_v_ptrs", C.c_void_p)]
+
+
+class RowqCache(C.Structure):
+    _fields_ = [("d_k_codes", C.c_void_p), ("d_v_codes", C.c_void_p), ("d_k_scales", C.c_void_p), ("d_v_scales", C.c_void_p),
+                ("seq_rows", C.c_uint64), ("d_page_table", C.c_void_p), ("page_rows", C.c_uint32),
+                ("max_pages_per_seq", C.c_uint32), ("num_pages", C.c_uint32), ("_pad", C.c_uint32)]
+
+
+class ScoreRuleC(C.Structure):
+    _fields_ = [("scale", C.c_float), ("cap", C.c_float), ("window", C.c_uint32), ("_pad", C.c_uint32),
+                ("d_slopes", C.c_void_p), ("d_prefix_lens", C.c_void_p), ("d_doc_start", C.c_void_p)]
 
 
 _lib = None
@@ -138,6 +151,16 @@ def load() -> C.CDLL:
     L.shady_gptq_matvec.argtypes = [vp, C.POINTER(GptqWeight), f32p, f32p, C.c_uint32]
     L.shady_qkv_proj_append.argtypes = [vp, C.POINTER(AppendParams), C.POINTER(GptqWeight), C.POINTER(GptqWeight),
                                         C.POINTER(GptqWeight), f32p, vp, f32p, C.POINTER(KvCache), vp, u32p, u32p, u32p]
+    L.shady_kv_append_rowq.argtypes = [vp, C.POINTER(AppendParams), vp, vp, vp, vp, f32p, vp, vp, C.POINTER(RowqCache), vp,
+                                       u32p, u32p, u32p, u32p, C.c_uint32]
+    L.shady_kv_read_rowq.argtypes = [vp, C.POINTER(RowqCache), C.c_uint32, C.c_uint32, C.c_uint32, u32p, u32p, C.c_uint32,
+                                     vp, vp, C.c_uint32]
+    L.shady_decode_rule_workspace_size.argtypes = [vp, C.POINTER(DecodeParams), C.POINTER(sz)]
+    L.shady_decode_rule_workspace_init.argtypes = [vp, C.POINTER(DecodeParams), vp, sz]
+    L.shady_attn_decode_rule.argtypes = [vp, C.POINTER(DecodeParams), C.POINTER(ScoreRuleC), vp, C.POINTER(KvCache),
+                                         C.POINTER(RowqCache), u32p, vp, f32p, vp, sz]
+    L.shady_attn_prefill_rule.argtypes = [vp, C.POINTER(PrefillParams), C.POINTER(ScoreRuleC), vp, C.POINTER(KvCache),
+                                          C.c_uint64, u32p, C.c_uint32, u32p, u32p, vp, f32p]
     L.shady_sigmoid_mul.argtypes = [vp, f32p, f32p, C.c_uint32]
     L.shady_fill_randn.argtypes = [vp, vp, C.c_uint64, C.c_uint32, C.c_uint64, C.c_uint64, C.c_uint64]
     for name in EXPORTS:

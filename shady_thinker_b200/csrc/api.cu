@@ -108,6 +108,17 @@ int launch_qkv_proj_append(shady_ctx *, const shady_append_params *, const shady
                            const uint32_t *, const uint32_t *, const uint32_t *);
 int launch_prefill_append(shady_ctx *, const shady_append_params *, const shady_prefill_params *, const void *, const void *,
                           const void *, const uint16_t *, const shady_kv_cache *, void *, void *, size_t);
+int launch_append_rowq(shady_ctx *, const shady_append_params *, const void *, const void *, const void *, void *, float *, void *, void *,
+                       const shady_rowq_cache *, const uint16_t *, const uint32_t *, const uint32_t *, const uint32_t *, const uint32_t *,
+                       uint32_t);
+int launch_read_rowq(shady_ctx *, const shady_rowq_cache *, uint32_t, uint32_t, uint32_t, const uint32_t *, const uint32_t *, uint32_t,
+                     void *, void *, uint32_t);
+int decode_rule_workspace_size(shady_ctx *, const shady_decode_params *, size_t *);
+int decode_rule_workspace_init(shady_ctx *, const shady_decode_params *, void *, size_t);
+int launch_decode_rule(shady_ctx *, const shady_decode_params *, const shady_score_rule *, const void *, const shady_kv_cache *,
+                       const shady_rowq_cache *, const uint32_t *, void *, float *, void *, size_t);
+int launch_prefill_rule(shady_ctx *, const shady_prefill_params *, const shady_score_rule *, const void *, const shady_kv_cache *, uint64_t,
+                        const uint32_t *, uint32_t, const uint32_t *, const uint32_t *, void *, float *);
 unsigned long long p2p_buffer_bytes(uint32_t world, uint32_t nh, uint32_t hd);
 int launch_combine_p2p(shady_ctx *, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, void *const *, const float *, void *,
                        uint32_t, const float *);
@@ -460,6 +471,46 @@ int shady_qkv_proj_append(shady_ctx *ctx, const shady_append_params *p, const sh
     CTX_ENTER(ctx);
     return launch_qkv_proj_append(ctx, p, wq, wk, wv, d_x, d_q_out, d_q_gate, cache, d_qk_norm_bf16, d_pos_start, d_pos_h,
                                   d_pos_w);
+}
+
+int shady_kv_append_rowq(shady_ctx *ctx, const shady_append_params *p, const void *d_q_proj_full, const void *d_k_proj,
+                         const void *d_v_proj, void *d_q_out, float *d_q_gate, void *d_k_out, void *d_v_out,
+                         const shady_rowq_cache *cache, const uint16_t *d_qk_norm_bf16, const uint32_t *d_pos_start,
+                         const uint32_t *d_pos_h, const uint32_t *d_pos_w, const uint32_t *d_tok_start, uint32_t total_tokens) {
+    CTX_ENTER(ctx);
+    return launch_append_rowq(ctx, p, d_q_proj_full, d_k_proj, d_v_proj, d_q_out, d_q_gate, d_k_out, d_v_out, cache, d_qk_norm_bf16,
+                              d_pos_start, d_pos_h, d_pos_w, d_tok_start, total_tokens);
+}
+
+int shady_kv_read_rowq(shady_ctx *ctx, const shady_rowq_cache *cache, uint32_t num_kv_heads, uint32_t head_dim, uint32_t num_seqs,
+                       const uint32_t *d_row_start, const uint32_t *d_out_start, uint32_t total_rows, void *d_k_out, void *d_v_out,
+                       uint32_t out_dtype) {
+    CTX_ENTER(ctx);
+    return launch_read_rowq(ctx, cache, num_kv_heads, head_dim, num_seqs, d_row_start, d_out_start, total_rows, d_k_out, d_v_out, out_dtype);
+}
+
+int shady_decode_rule_workspace_size(shady_ctx *ctx, const shady_decode_params *p, size_t *bytes) {
+    CTX_ENTER(ctx);
+    return decode_rule_workspace_size(ctx, p, bytes);
+}
+
+int shady_decode_rule_workspace_init(shady_ctx *ctx, const shady_decode_params *p, void *d_workspace, size_t workspace_bytes) {
+    CTX_ENTER(ctx);
+    return decode_rule_workspace_init(ctx, p, d_workspace, workspace_bytes);
+}
+
+int shady_attn_decode_rule(shady_ctx *ctx, const shady_decode_params *p, const shady_score_rule *rule, const void *d_q,
+                           const shady_kv_cache *cache, const shady_rowq_cache *rowq, const uint32_t *d_seq_lens, void *d_out,
+                           float *d_lse, void *d_workspace, size_t workspace_bytes) {
+    CTX_ENTER(ctx);
+    return launch_decode_rule(ctx, p, rule, d_q, cache, rowq, d_seq_lens, d_out, d_lse, d_workspace, workspace_bytes);
+}
+
+int shady_attn_prefill_rule(shady_ctx *ctx, const shady_prefill_params *p, const shady_score_rule *rule, const void *d_q,
+                            const shady_kv_cache *cache, uint64_t cache_rows, const uint32_t *d_q_starts, uint32_t total_q,
+                            const uint32_t *d_kv_starts, const uint32_t *d_kv_lens, void *d_out, float *d_lse) {
+    CTX_ENTER(ctx);
+    return launch_prefill_rule(ctx, p, rule, d_q, cache, cache_rows, d_q_starts, total_q, d_kv_starts, d_kv_lens, d_out, d_lse);
 }
 
 int shady_sigmoid_mul(shady_ctx *ctx, float *d_x, const float *d_gate, uint32_t n) {

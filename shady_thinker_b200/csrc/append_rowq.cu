@@ -1,0 +1,388 @@
+// The row-scaled 8-bit KV cache: the append that quantises rows as it writes them, and the read-back.
+//
+// append: per token and head, with x the projected row of head_dim values,
+//     Q, K:  x <- x * (1 + w) / sqrt(mean(x^2) + eps);  (x_a, x_b) <- rotation of every rotary pair by its angle
+//            (the arithmetic of fused_split_qknorm_kvstore.wgsl:126-218, angles rounded to f32 as there)
+//     K, V:  scale = clamp(max|x| / 127, 2^-60, 2^60), code = clamp(rne(x / scale), -127, 127), stored as code + 128
+// read:   value = (byte - 128) * scale, rounded once to the output type.
+//
+// Both are bound by memory once there are more than a few hundred rows, and by launch latency below that.
+#include "rowq.cuh"
+
+namespace shady {
+
+int fill_rowq_addr(shady_ctx *ctx, const shady_rowq_cache *cache, const char *who, RowqAddr *out) {
+    const std::string w(who);
+    SHADY_REQUIRE(ctx, cache, SHADY_ERR_BAD_ARG, w + ": null cache");
+    SHADY_REQUIRE(ctx, cache->d_k_codes && cache->d_v_codes && cache->d_k_scales && cache->d_v_scales, SHADY_ERR_BAD_ARG,
+                  w + ": a row-scaled cache needs code and scale arrays for K and V");
+    SHADY_REQUIRE(ctx, ((uintptr_t)cache->d_k_codes & 15) == 0 && ((uintptr_t)cache->d_v_codes & 15) == 0, SHADY_ERR_BAD_ARG,
+                  w + ": code arrays must be 16-byte aligned");
+    SHADY_REQUIRE(ctx, ((uintptr_t)cache->d_k_scales & 3) == 0 && ((uintptr_t)cache->d_v_scales & 3) == 0, SHADY_ERR_BAD_ARG,
+                  w + ": scale arrays must be 4-byte aligned");
+    RowqAddr a{};
+    a.k_codes = (unsigned char *)cache->d_k_codes; a.v_codes = (unsigned char *)cache->d_v_codes;
+    a.k_scales = cache->d_k_scales; a.v_scales = cache->d_v_scales;
+    if (cache->d_page_table) {
+        SHADY_REQUIRE(ctx, cache->page_rows && cache->page_rows % 16 == 0 && cache->max_pages_per_seq, SHADY_ERR_BAD_ARG,
+                      w + ": page_rows must be a positive multiple of 16 and max_pages_per_seq positive");
+        a.page_table = cache->d_page_table;
+        a.page_rows = cache->page_rows; a.max_pages = cache->max_pages_per_seq; a.num_pages = cache->num_pages;
+    } else {
+        SHADY_REQUIRE(ctx, cache->seq_rows, SHADY_ERR_BAD_ARG, w + ": seq_rows is zero");
+        a.seq_rows = cache->seq_rows;
+    }
+    *out = a;
+    return SHADY_OK;
+}
+
+// ---- vector loads and stores of N consecutive elements (N = 2, 4 or 8), as f32 -------------------------------------
+template <int BYTES> struct RawVec;
+template <> struct RawVec<2> { using type = unsigned short; };
+template <> struct RawVec<4> { using type = uint32_t; };
+template <> struct RawVec<8> { using type = uint2; };
+template <> struct RawVec<16> { using type = uint4; };
+template <> struct RawVec<32> { struct alignas(16) type { uint4 a, b; }; };
+
+template <typename T, int N> __device__ __forceinline__ void vec_cvt(const typename RawVec<N * sizeof(T)>::type &raw, float (&v)[N]) {
+    const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f32<T>(e[i]);
+}
+template <typename T, int N> __device__ __forceinline__ void vec_store(T *dst, const float (&v)[N]) {
+    typename RawVec<N * sizeof(T)>::type raw;
+    T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = from_f32<T>(v[i]);
+    *reinterpret_cast<typename RawVec<N * sizeof(T)>::type *>(dst) = raw;
+}
+template <int N> __device__ __forceinline__ void vec_store_dt(void *dst, size_t i, uint32_t dt, const float (&v)[N]) {
+    if (dt == SHADY_F32) vec_store<float, N>(reinterpret_cast<float *>(dst) + i, v);
+    else if (dt == SHADY_F16) vec_store<__half, N>(reinterpret_cast<__half *>(dst) + i, v);
+    else vec_store<__nv_bfloat16, N>(reinterpret_cast<__nv_bfloat16 *>(dst) + i, v);
+}
+
+struct AppendRowqArgs {
+    const void *q, *k, *v;
+    void *q_out, *k_out, *v_out;
+    float *gate;
+    RowqAddr cache;
+    const uint16_t *norm_w;
+    const uint32_t *pos_start, *pos_h, *pos_w, *tok_start;
+    uint32_t num_seqs, tokens_per_seq, total_tokens;
+    uint32_t nh, nkv, has_gate, q_dtype;
+    uint32_t chunks, per_chunk;   // a token's head vectors (Q heads, K heads, V heads) are dealt to `chunks` warps
+    uint32_t rd, s1, s2;
+    float eps;
+    float inv_freq[128];
+};
+
+constexpr uint32_t kAppendWarps = 8;
+
+// One warp takes per_chunk consecutive head vectors of one token; a lane holds HD/32 consecutive elements of each, so a
+// vector is one coalesced access, sums and maxima are five shuffles, and the lane's cos/sin serve all its vectors.
+// INTERLEAVED pairs (2i, 2i+1) lie in one lane; pairs (i, i + rd/2) meet through a row of shared memory per warp.
+template <typename T, int HD, bool INTERLEAVED>
+__global__ void __launch_bounds__(kAppendWarps * 32) append_rowq_kernel(const __grid_constant__ AppendRowqArgs a) {
+    constexpr int N = HD / 32;
+    constexpr int NP = INTERLEAVED ? N / 2 : N;   // angles a lane needs
+    using Raw = typename RawVec<N * sizeof(T)>::type;
+    __shared__ float sm_freq[128];
+    __shared__ float sm_row[INTERLEAVED ? 1 : kAppendWarps][INTERLEAVED ? 1 : HD];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (uint32_t i = threadIdx.x; i < a.rd / 2; i += kAppendWarps * 32) sm_freq[i] = a.inv_freq[i];
+    __syncthreads();
+
+    const unsigned long long unit = (unsigned long long)blockIdx.x * kAppendWarps + warp;
+    const uint32_t tok = (uint32_t)(unit / a.chunks);
+    const uint32_t limit = a.tok_start ? min(a.total_tokens, __ldg(a.tok_start + a.num_seqs)) : a.total_tokens;
+    if (tok >= limit) return;
+    const uint32_t nvec = a.nh + 2 * a.nkv;
+    const uint32_t i0 = (uint32_t)(unit % a.chunks) * a.per_chunk, i1 = min(i0 + a.per_chunk, nvec);
+
+    const uint32_t qstride = a.has_gate ? 2 * HD : HD;
+    const uint32_t d0 = lane * N;
+    auto src = [&](uint32_t i) -> const T * {   // head vector i of this token
+        if (i < a.nh) return reinterpret_cast<const T *>(a.q) + ((size_t)tok * a.nh + i) * qstride + d0;
+        if (i < a.nh + a.nkv) return reinterpret_cast<const T *>(a.k) + ((size_t)tok * a.nkv + (i - a.nh)) * HD + d0;
+        return reinterpret_cast<const T *>(a.v) + ((size_t)tok * a.nkv + (i - a.nh - a.nkv)) * HD + d0;
+    };
+    // vectors are requested kAhead before their use, the first ones before anything else of the token is known
+    constexpr int kAhead = 3;
+    Raw next[kAhead], gnext[kAhead];
+    auto request = [&](uint32_t i, Raw &r, Raw &g) {
+        if (i >= i1) return;
+        r = *reinterpret_cast<const Raw *>(src(i));
+        if (a.has_gate && i < a.nh) g = *reinterpret_cast<const Raw *>(src(i) + HD);
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) request(i0 + u, next[u], gnext[u]);
+
+    uint32_t seq, j;
+    if (a.tok_start) {
+        seq = warp_find_seq(a.tok_start, a.num_seqs, tok, lane);
+        j = tok - __ldg(a.tok_start + seq);
+    } else {
+        seq = tok / a.tokens_per_seq;
+        j = tok - seq * a.tokens_per_seq;
+    }
+    const uint32_t pos = __ldg(a.pos_start + seq) + j;
+    unsigned long long row = 0;
+    const bool have_row = i1 > a.nh && rowq_row(a.cache, seq, pos, row);
+    float cs[NP], sn[NP];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) { cs[p] = 1.f; sn[p] = 0.f; }
+    if (i0 < a.nh + a.nkv) {   // (a warp with V heads only has nothing to rotate)
+        const uint32_t p_h = a.pos_h ? __ldg(a.pos_h + seq) + j : pos, p_w = a.pos_w ? __ldg(a.pos_w + seq) + j : pos;
+        const uint32_t half = a.rd / 2;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const uint32_t d = d0 + (INTERLEAVED ? 2 * p : p);
+            if (d < a.rd) {
+                const uint32_t i = INTERLEAVED ? d / 2 : (d < half ? d : d - half);
+                uint32_t at = pos;
+                if ((i % 3u) == 1u && i < a.s1) at = p_h;
+                else if ((i % 3u) == 2u && i < a.s2) at = p_w;
+                sincosf((float)at * sm_freq[i], &sn[p], &cs[p]);
+                if (!INTERLEAVED && d < half) sn[p] = -sn[p];   // x cos - y sin below, y cos + x sin above
+            }
+        }
+    }
+
+    for (uint32_t ib = i0; ib < i1; ib += kAhead) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const uint32_t i = ib + u;
+            if (i >= i1) break;
+            float x[N];
+            vec_cvt<T, N>(next[u], x);
+            float gt[N];
+            const bool is_q = i < a.nh, is_v = i >= a.nh + a.nkv;
+            if (a.has_gate && is_q) vec_cvt<T, N>(gnext[u], gt);
+            request(i + kAhead, next[u], gnext[u]);
+            if (!is_v) {
+                if (a.norm_w) {
+                    float ssq = 0.f;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) ssq += x[e] * x[e];
+                    const float rms = 1.0f / sqrtf(warp_sum(ssq) / (float)HD + a.eps);
+                    typename RawVec<N * 2>::type wraw = *reinterpret_cast<const typename RawVec<N * 2>::type *>(a.norm_w + (is_q ? 0 : HD) + d0);
+                    float w[N];
+                    vec_cvt<__nv_bfloat16, N>(wraw, w);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) x[e] = x[e] * rms * (1.0f + w[e]);
+                }
+                if (a.rd) {
+                    if constexpr (INTERLEAVED) {
+#pragma unroll
+                        for (int p = 0; p < NP; ++p) {
+                            const float c = x[2 * p], d = x[2 * p + 1];
+                            x[2 * p] = c * cs[p] - d * sn[p];
+                            x[2 * p + 1] = d * cs[p] + c * sn[p];
+                        }
+                    } else {
+                        float *rowp = sm_row[warp];
+                        __syncwarp();
+#pragma unroll
+                        for (int e = 0; e < N; ++e) rowp[d0 + e] = x[e];
+                        __syncwarp();
+                        const uint32_t half = a.rd / 2;
+#pragma unroll
+                        for (int e = 0; e < N; ++e) {
+                            const uint32_t d = d0 + e;
+                            if (d < a.rd) x[e] = x[e] * cs[e] + rowp[d < half ? d + half : d - half] * sn[e];
+                        }
+                    }
+                }
+            }
+            if (is_q) {
+                const size_t o = ((size_t)tok * a.nh + i) * HD + d0;
+                vec_store_dt<N>(a.q_out, o, a.q_dtype, x);
+                if (a.has_gate && a.gate) vec_store<float, N>(a.gate + o, gt);
+                continue;
+            }
+            const uint32_t kvh = i - a.nh - (is_v ? a.nkv : 0u);
+            float amax = 0.f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) amax = fmaxf(amax, fabsf(x[e]));
+            const float scale = rowq_scale(warp_max(amax)), inv = 1.0f / scale;
+            alignas(8) unsigned char code[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int c = rowq_code(x[e], inv);
+                code[e] = (unsigned char)(c + 128);
+                x[e] = (float)c * scale;
+            }
+            if (have_row) {
+                const unsigned long long at = row * a.nkv + kvh;
+                *reinterpret_cast<typename RawVec<N>::type *>((is_v ? a.cache.v_codes : a.cache.k_codes) + at * HD + d0) =
+                    *reinterpret_cast<const typename RawVec<N>::type *>(code);
+                if (lane == 0) (is_v ? a.cache.v_scales : a.cache.k_scales)[at] = scale;
+            }
+            if (a.k_out) vec_store_dt<N>(is_v ? a.v_out : a.k_out, ((size_t)tok * a.nkv + kvh) * HD + d0, a.q_dtype, x);
+        }
+    }
+}
+
+int launch_append_rowq(shady_ctx *ctx, const shady_append_params *p, const void *d_q, const void *d_k, const void *d_v, void *d_q_out,
+                       float *d_gate, void *d_k_out, void *d_v_out, const shady_rowq_cache *cache, const uint16_t *norm_w,
+                       const uint32_t *d_pos_start, const uint32_t *d_pos_h, const uint32_t *d_pos_w, const uint32_t *d_tok_start,
+                       uint32_t total_tokens) {
+    SHADY_REQUIRE(ctx, p && d_q && d_k && d_v && d_q_out && cache && d_pos_start, SHADY_ERR_BAD_ARG, "kv_append_rowq: null argument");
+    SHADY_REQUIRE(ctx, p->num_heads && p->num_kv_heads && p->num_seqs, SHADY_ERR_BAD_ARG, "kv_append_rowq: zero-sized problem");
+    SHADY_REQUIRE(ctx, p->num_heads <= 65536 && p->num_kv_heads <= 65536, SHADY_ERR_UNSUPPORTED, "kv_append_rowq: too many heads");
+    SHADY_REQUIRE(ctx, p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256, SHADY_ERR_UNSUPPORTED,
+                  "kv_append_rowq: head_dim must be 64, 128 or 256");
+    SHADY_REQUIRE(ctx, p->rotary_dim <= p->head_dim && p->rotary_dim % 2 == 0, SHADY_ERR_BAD_ARG,
+                  "kv_append_rowq: rotary_dim must be even and <= head_dim");
+    SHADY_REQUIRE(ctx, p->in_dtype <= SHADY_BF16 && p->q_dtype <= SHADY_BF16, SHADY_ERR_BAD_ARG, "kv_append_rowq: bad dtype");
+    SHADY_REQUIRE(ctx, !p->write_k_back, SHADY_ERR_UNSUPPORTED, "kv_append_rowq: write_k_back is not supported (d_k_out has the stored rows)");
+    SHADY_REQUIRE(ctx, !p->has_gate || d_gate, SHADY_ERR_BAD_ARG, "kv_append_rowq: has_gate needs d_q_gate");
+    SHADY_REQUIRE(ctx, !d_k_out == !d_v_out, SHADY_ERR_BAD_ARG, "kv_append_rowq: d_k_out and d_v_out are given together or not at all");
+    for (const void *ptr : {d_q, d_k, d_v, (const void *)d_q_out, (const void *)d_gate, (const void *)d_k_out, (const void *)d_v_out, (const void *)norm_w})
+        SHADY_REQUIRE(ctx, ((uintptr_t)ptr & 15) == 0, SHADY_ERR_BAD_ARG, "kv_append_rowq: tensors must be 16-byte aligned");
+    AppendRowqArgs a{};
+    if (const int st = fill_rowq_addr(ctx, cache, "kv_append_rowq", &a.cache)) return st;
+    if (!d_tok_start) {
+        SHADY_REQUIRE(ctx, p->tokens_per_seq, SHADY_ERR_BAD_ARG, "kv_append_rowq: tokens_per_seq is zero");
+        const unsigned long long n = (unsigned long long)p->num_seqs * p->tokens_per_seq;
+        SHADY_REQUIRE(ctx, n <= 0xffffffffull && total_tokens == n, SHADY_ERR_BAD_ARG,
+                      "kv_append_rowq: total_tokens is not num_seqs * tokens_per_seq");
+    } else if (!total_tokens) {
+        return SHADY_OK;
+    }
+    a.q = d_q; a.k = d_k; a.v = d_v; a.q_out = d_q_out; a.k_out = d_k_out; a.v_out = d_v_out; a.gate = d_gate;
+    a.norm_w = norm_w; a.pos_start = d_pos_start; a.pos_h = d_pos_h; a.pos_w = d_pos_w; a.tok_start = d_tok_start;
+    a.num_seqs = p->num_seqs; a.tokens_per_seq = p->tokens_per_seq; a.total_tokens = total_tokens;
+    a.nh = p->num_heads; a.nkv = p->num_kv_heads; a.has_gate = p->has_gate ? 1u : 0u; a.q_dtype = p->q_dtype;
+    a.rd = p->rotary_dim; a.s1 = p->s1_limit; a.s2 = p->s2_limit; a.eps = p->eps;
+    for (uint32_t i = 0; i < p->rotary_dim / 2; ++i)   // the libm call the 16-bit append and the oracle make
+        a.inv_freq[i] = 1.0f / powf(p->rope_theta, 2.0f * (float)i / (float)p->rotary_dim);
+    // A warp serves as many vectors of its token as still leave every SM about 48 warps: one each for a decode step,
+    // where the launch is latency, the whole token for a prompt, where the angles are then computed once.
+    const uint32_t nvec = a.nh + 2 * a.nkv;
+    const unsigned long long all = (unsigned long long)total_tokens * nvec, room = (unsigned long long)ctx->num_sms * 48;
+    unsigned long long per = all / room;
+    per = per < 1 ? 1 : (per > nvec ? nvec : per);
+    a.chunks = (uint32_t)((nvec + per - 1) / per);
+    a.per_chunk = (nvec + a.chunks - 1) / a.chunks;
+    a.chunks = (nvec + a.per_chunk - 1) / a.per_chunk;
+    const unsigned long long blocks = ((unsigned long long)total_tokens * a.chunks + kAppendWarps - 1) / kAppendWarps;
+    SHADY_REQUIRE(ctx, blocks <= 0x7fffffffull, SHADY_ERR_UNSUPPORTED, "kv_append_rowq: too many tokens for one launch");
+    auto go = [&](auto kern) { kern<<<(unsigned)blocks, kAppendWarps * 32, 0, ctx->stream>>>(a); };
+    auto by_dim = [&](auto t) {
+        using T = decltype(t);
+        if (p->interleaved) {
+            if (p->head_dim == 64) go(append_rowq_kernel<T, 64, true>);
+            else if (p->head_dim == 128) go(append_rowq_kernel<T, 128, true>);
+            else go(append_rowq_kernel<T, 256, true>);
+        } else {
+            if (p->head_dim == 64) go(append_rowq_kernel<T, 64, false>);
+            else if (p->head_dim == 128) go(append_rowq_kernel<T, 128, false>);
+            else go(append_rowq_kernel<T, 256, false>);
+        }
+    };
+    if (p->in_dtype == SHADY_F32) by_dim(float{});
+    else if (p->in_dtype == SHADY_F16) by_dim(__half{});
+    else by_dim(__nv_bfloat16{});
+    ctx->launches++;
+    SHADY_CUDA_OK(ctx, cudaGetLastError());
+    return SHADY_OK;
+}
+
+// ---- read-back -----------------------------------------------------------------------------------------------------
+struct ReadRowqArgs {
+    RowqAddr cache;
+    const uint32_t *row_start, *out_start;
+    void *k_out, *v_out;
+    uint32_t num_seqs, total_rows, nkv, hd, rows_per_block;
+};
+constexpr uint32_t kReadThreads = 256, kReadMaxRows = 64;
+
+// A block reads rows_per_block packed rows: its warps look the rows up (one 32-way search each) into shared memory, then
+// all threads stream 16-code pieces of K and V, kUnroll in flight per thread, every access coalesced.
+template <typename T>
+__global__ void __launch_bounds__(kReadThreads) read_rowq_kernel(const __grid_constant__ ReadRowqArgs a) {
+    __shared__ unsigned long long sm_row[kReadMaxRows];
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t limit = min(a.total_rows, __ldg(a.out_start + a.num_seqs));
+    const uint32_t r0 = blockIdx.x * a.rows_per_block;
+    if (r0 >= limit) return;
+    const uint32_t nr = min(a.rows_per_block, limit - r0);
+    for (uint32_t r = warp; r < nr; r += kReadThreads / 32) {
+        const uint32_t s = warp_find_seq(a.out_start, a.num_seqs, r0 + r, lane);
+        const uint32_t pos = (a.row_start ? __ldg(a.row_start + s) : 0u) + (r0 + r - __ldg(a.out_start + s));
+        unsigned long long row = ~0ull;
+        if (!rowq_row(a.cache, s, pos, row)) row = ~0ull;
+        if (lane == 0) sm_row[r] = row;
+    }
+    __syncthreads();
+    const uint32_t row_pieces = a.nkv * a.hd / 16, head_pieces = a.hd / 16;
+    const uint32_t n = nr * row_pieces;
+    const unsigned char *codes = blockIdx.y ? a.cache.v_codes : a.cache.k_codes;
+    const float *scales = blockIdx.y ? a.cache.v_scales : a.cache.k_scales;
+    T *out = reinterpret_cast<T *>(blockIdx.y ? a.v_out : a.k_out);
+    if (!out) return;
+    constexpr uint32_t kUnroll = 4;
+    for (uint32_t i0 = tid; i0 < n; i0 += kReadThreads * kUnroll) {
+        uint4 c[kUnroll];
+        float s[kUnroll];
+#pragma unroll
+        for (uint32_t u = 0; u < kUnroll; ++u) {
+            const uint32_t i = i0 + u * kReadThreads;
+            c[u] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);   // code 0
+            s[u] = 0.f;
+            if (i < n) {
+                const unsigned long long row = sm_row[i / row_pieces];
+                const uint32_t piece = i % row_pieces;
+                if (row != ~0ull) {
+                    c[u] = __ldcs(reinterpret_cast<const uint4 *>(codes + row * a.nkv * a.hd) + piece);
+                    s[u] = __ldg(scales + row * a.nkv + piece / head_pieces);
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kUnroll; ++u) {
+            const uint32_t i = i0 + u * kReadThreads;
+            if (i >= n) break;
+            const unsigned char *b = reinterpret_cast<const unsigned char *>(&c[u]);
+            alignas(16) T v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = from_f32<T>((float)((int)b[e] - 128) * s[u]);
+            uint4 *dst = reinterpret_cast<uint4 *>(out + ((size_t)r0 * row_pieces + i) * 16);
+#pragma unroll
+            for (int e = 0; e < (int)sizeof(T); ++e) dst[e] = reinterpret_cast<const uint4 *>(v)[e];
+        }
+    }
+}
+
+int launch_read_rowq(shady_ctx *ctx, const shady_rowq_cache *cache, uint32_t nkv, uint32_t hd, uint32_t num_seqs,
+                     const uint32_t *d_row_start, const uint32_t *d_out_start, uint32_t total_rows, void *d_k_out, void *d_v_out,
+                     uint32_t out_dtype) {
+    SHADY_REQUIRE(ctx, cache && d_out_start && (d_k_out || d_v_out), SHADY_ERR_BAD_ARG, "kv_read_rowq: null argument");
+    SHADY_REQUIRE(ctx, nkv && num_seqs, SHADY_ERR_BAD_ARG, "kv_read_rowq: zero-sized problem");
+    SHADY_REQUIRE(ctx, hd == 64 || hd == 128 || hd == 256, SHADY_ERR_UNSUPPORTED, "kv_read_rowq: head_dim must be 64, 128 or 256");
+    SHADY_REQUIRE(ctx, nkv <= 65536, SHADY_ERR_UNSUPPORTED, "kv_read_rowq: too many heads");
+    SHADY_REQUIRE(ctx, out_dtype <= SHADY_BF16, SHADY_ERR_BAD_ARG, "kv_read_rowq: bad output dtype");
+    SHADY_REQUIRE(ctx, ((uintptr_t)d_k_out & 15) == 0 && ((uintptr_t)d_v_out & 15) == 0, SHADY_ERR_BAD_ARG,
+                  "kv_read_rowq: outputs must be 16-byte aligned");
+    ReadRowqArgs a{};
+    if (const int st = fill_rowq_addr(ctx, cache, "kv_read_rowq", &a.cache)) return st;
+    if (!total_rows) return SHADY_OK;
+    a.row_start = d_row_start; a.out_start = d_out_start; a.k_out = d_k_out; a.v_out = d_v_out;
+    a.num_seqs = num_seqs; a.total_rows = total_rows; a.nkv = nkv; a.hd = hd;
+    // rows of a block: about 32 KB of codes of one tensor, fewer while the grid would leave SMs without a block
+    uint32_t rows = 32768u / (nkv * hd);
+    rows = rows < 1 ? 1 : (rows > kReadMaxRows ? kReadMaxRows : rows);
+    while (rows > 1 && (total_rows + rows - 1) / rows < (uint32_t)ctx->num_sms * 4) rows = (rows + 1) / 2;
+    a.rows_per_block = rows;
+    const dim3 grid((total_rows + rows - 1) / rows, 2);
+    if (out_dtype == SHADY_F32) read_rowq_kernel<float><<<grid, kReadThreads, 0, ctx->stream>>>(a);
+    else if (out_dtype == SHADY_F16) read_rowq_kernel<__half><<<grid, kReadThreads, 0, ctx->stream>>>(a);
+    else read_rowq_kernel<__nv_bfloat16><<<grid, kReadThreads, 0, ctx->stream>>>(a);
+    ctx->launches++;
+    SHADY_CUDA_OK(ctx, cudaGetLastError());
+    return SHADY_OK;
+}
+
+}  // namespace shady

@@ -1,0 +1,596 @@
+// Attention of one new token per sequence under a score rule, over 16-bit caches and over the row-scaled 8-bit cache.
+//
+// With q the query of head h at position i = L - 1, and the rows j that the rule lets it see (shady_score_rule):
+//     z_j = cap * tanh(q.k_j * scale / cap) - slope_h * (i - j)          (cap and slope as the rule has them)
+//     out = sum_j e^(z_j) v_j / sum_j e^(z_j),          lse = ln sum_j e^(z_j)
+// and for the row-scaled cache k_j = kc_j * ks_j, v_j = vc_j * vs_j with codes kc, vc and the row's scales ks, vs.
+//
+// What bounds it: every visible cache row is read once, 2..4 operations per byte and head, so memory does once there
+// are enough rows; below that the launch and the dependent loads of its start.
+//
+//   * All visible 16-row blocks of all (sequence, kv head, group of eight query heads) lie end to end on one line, which
+//     is cut into equal shares for a resident grid.  The CTAs work the shares out from the lengths in device memory,
+//     so nothing is planned on the host and a captured launch serves growing sequences.  A window or a document start
+//     leaves only the blocks with a visible row on the line; prefix rows in front of a window are blocks of their own.
+//   * A warp streams its own blocks with 16-byte cp.async into a ring of its own (rows that are not visible are
+//     filled with zeros and not read), the positions on the M rows of the MMA and eight heads on its N columns:
+//     S^T = K Q^T, O^T = V^T P^T, softmax statistics in f32 by shuffles.  Each cache byte is read once per eight heads.
+//   * Codes become f16 without a conversion instruction: a byte permute puts the byte c + 128 under 0x64, which is the
+//     f16 1024 + c + 128, and one subtraction of 1152 leaves c exactly.  ks multiplies the score; vs goes into the
+//     weight, whose running maximum is taken over z + ln(vs), so that the f16 weights stay within [0, 1] whatever
+//     the sizes of the scales; the sum of e^z divides by vs again in f32.
+//   * A share that holds only part of a (sequence, kv head, group) writes a record; the CTA that arrives last at its
+//     counter joins the records in the order of the shares, so the result does not depend on which CTA it was.
+#include <type_traits>
+
+#include "rowq.cuh"
+#include "rule.cuh"
+
+namespace shady {
+
+int fill_rule(shady_ctx *ctx, const shady_score_rule *rule, uint32_t head_dim, const char *who, RuleArgs *out) {
+    const std::string w(who);
+    RuleArgs r{};
+    r.scale = 1.0f / sqrtf((float)head_dim);
+    if (rule) {
+        SHADY_REQUIRE(ctx, rule->scale >= 0.f && isfinite(rule->scale), SHADY_ERR_BAD_ARG, w + ": scale must be finite and not negative");
+        SHADY_REQUIRE(ctx, rule->cap >= 0.f && isfinite(rule->cap), SHADY_ERR_BAD_ARG, w + ": cap must be finite and not negative");
+        if (rule->scale > 0.f) r.scale = rule->scale;
+        if (rule->cap > 0.f) {
+            r.cap = rule->cap; r.inv_cap = 1.0f / rule->cap;
+            SHADY_REQUIRE(ctx, isfinite(r.inv_cap) && r.inv_cap > 0.f, SHADY_ERR_BAD_ARG, w + ": cap is too small or too large");
+        }
+        r.window = rule->window; r.slopes = rule->d_slopes; r.prefix = rule->d_prefix_lens; r.doc = rule->d_doc_start;
+    }
+    *out = r;
+    return SHADY_OK;
+}
+
+namespace dr {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32, kBlock = 16, kHeads = 8;
+constexpr uint32_t kMinShare = kWarps;   // blocks: one per warp
+
+struct Args {
+    RuleArgs rule;
+    KvAddr kv;         // 16-bit cache
+    RowqAddr rq;       // row-scaled cache
+    const void *q;
+    void *out;
+    float *lse;
+    const uint32_t *lens;
+    uint32_t *counters;   // [num_seqs][nkv * groups]
+    float *records;       // [2 * grid][kHeads][HD + 2]
+    uint32_t num_seqs, nkv, G, nh, groups, q_dtype, out_dtype;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool ok) {   // !ok: 16 bytes of zeros, nothing read
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0));
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0));
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
+    return d;
+}
+template <typename T> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (!std::is_same<T, __nv_bfloat16>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+// bytes SEL & 0xf and SEL >> 4 of x, each a code + 128, as the f16 pair of the codes
+template <uint32_t SEL> __device__ __forceinline__ uint32_t codes_to_f16(uint32_t x) {
+    const uint32_t w = __byte_perm(x, 0x64646464u, 0x4040u | (SEL & 0xfu) | ((SEL >> 4) << 8));
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6480)));   // 0x6480 = 1152
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+template <int HD, bool Q8> struct Smem {
+    static constexpr int kRow = HD * (Q8 ? 1 : 2);           // one kv head's part of a cache row
+    static constexpr int kTile = kBlock * kRow;
+    // 16-byte chunk c of row r lies in place c ^ swz(r): the eight rows of an ldmatrix then fall on different banks
+    static __device__ __forceinline__ uint32_t swz(uint32_t r) { return kRow >= 128 ? r & 7 : (r >> 1) & 3; }
+    static constexpr int kScales = Q8 ? 2 * kBlock * 4 : 0;  // the block's K scales, then its V scales
+    static constexpr int kStage = 2 * kTile + kScales;
+    // stages of a warp's ring: with the CTAs an SM then holds (kCtas), 96..192 KB of an SM's rows are in flight
+    static constexpr int kStages = kStage >= 16384 ? 3 : (kStage >= 8192 ? 3 : 4);
+    static constexpr int kCtas = kStage >= 16384 ? 1 : (kStage >= 8192 ? 2 : 3);
+    static constexpr int kQ = kHeads * HD * 2;
+    static constexpr int kORow = HD + 4;                     // floats of a head's row in a warp's merge tile
+    static constexpr int kMergeTile = kHeads * kORow * 4;
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kMisc = 2 * kWarps * kHeads * 4 + kHeads * 4 + 16;
+    static constexpr int kTotal = kQ + kRing + kMisc;
+    static_assert(kWarps * kMergeTile <= kRing, "the merge tiles reuse the rings");
+};
+
+// What one sequence puts on the line.
+struct Seq {
+    uint32_t L, doc, wlo, pre;   // rows; first visible row; first row of the window; prefix rows
+    uint32_t a0, na, b0, n;      // prefix blocks a0 .. a0+na-1, then window blocks b0 ..; n in all (at least 1)
+};
+__device__ __forceinline__ Seq seq_of(const Args &a, uint32_t s) {
+    Seq q;
+    q.L = __ldg(a.lens + s);
+    q.doc = a.rule.doc ? __ldg(a.rule.doc + s) : 0u;
+    q.pre = a.rule.prefix ? min(__ldg(a.rule.prefix + s), q.L) : 0u;
+    q.wlo = max(q.doc, a.rule.window && q.L > a.rule.window ? q.L - a.rule.window : 0u);
+    q.a0 = q.doc / kBlock; q.na = 0;
+    q.b0 = q.wlo / kBlock;
+    uint32_t nb = 0;
+    if (q.wlo < q.L) nb = (q.L - 1) / kBlock - q.b0 + 1;
+    const uint32_t pe = min(q.pre, q.wlo);
+    if (q.doc < pe) q.na = min((pe - 1) / kBlock + 1, nb ? q.b0 : ~0u) - q.a0;   // a block that both parts touch counts as the window's
+    q.n = max(1u, q.na + nb);
+    return q;
+}
+__device__ __forceinline__ bool visible(const Seq &q, uint32_t row) { return row < q.L && row >= q.doc && (row >= q.wlo || row < q.pre); }
+
+template <typename T, int HD, bool Q8>
+__global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_kernel(const __grid_constant__ Args a) {
+    using S = Smem<HD, Q8>;
+    constexpr int ST = S::kStages;
+    constexpr int CH = S::kRow / 16;                  // 16-byte chunks of a row
+    constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;    // rows per warp-wide copy
+    constexpr int NI = kBlock / RPI;
+    extern __shared__ __align__(128) unsigned char smem[];
+    unsigned char *sm_q = smem, *sm_ring = smem + S::kQ;
+    float *sm_m = reinterpret_cast<float *>(smem + S::kQ + S::kRing), *sm_l = sm_m + kWarps * kHeads, *sm_qs = sm_l + kWarps * kHeads;
+    uint32_t *sm_flag = reinterpret_cast<uint32_t *>(sm_qs + kHeads);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t g = lane >> 2, t = lane & 3, mat = lane >> 3, rin = lane & 7;
+    const uint32_t U = a.nkv * a.groups;
+
+    // ---- this CTA's share of the line; every warp works it out for itself ----
+    uint32_t total = 0;
+    for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += 32) {
+        const uint32_t s = s0 + lane;
+        total += __reduce_add_sync(0xffffffffu, s < a.num_seqs ? seq_of(a, s).n * U : 0u);
+    }
+    const uint32_t share = max((total + gridDim.x - 1) / gridDim.x, kMinShare);
+    uint32_t x = blockIdx.x * share;
+    const uint32_t x_first = x, x_end = min(x + share, total);
+    if (x >= x_end) return;
+    uint32_t seq = 0, base = 0;   // the sequence that holds x, and where it starts on the line
+    for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += 32) {
+        const uint32_t s = s0 + lane;
+        const uint32_t n = s < a.num_seqs ? seq_of(a, s).n * U : 0u;
+        uint32_t upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= (uint32_t)o) upto += v;
+        }
+        const uint32_t all = __shfl_sync(0xffffffffu, upto, 31);
+        if (x < base + all) {
+            const uint32_t k = __ffs(__ballot_sync(0xffffffffu, x < base + upto)) - 1;
+            seq = s0 + k;
+            base += __shfl_sync(0xffffffffu, upto - n, k);
+            break;
+        }
+        base += all;
+    }
+
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm_ring) + warp * ST * S::kStage;
+    const uint32_t q_addr = (uint32_t)__cvta_generic_to_shared(sm_q);
+    while (x < x_end) {
+        const Seq sq = seq_of(a, seq);
+        const uint32_t unit = (x - base) / sq.n, u0 = base + unit * sq.n, u1 = u0 + sq.n;   // (kv head, head group) on the line
+        const uint32_t p0 = x - u0, p1 = min(x_end, u1) - u0;                               // blocks [p0, p1) of it are this piece
+        const bool whole = p1 - p0 == sq.n;
+        const uint32_t kvh = unit / a.groups, grp = unit % a.groups;
+        const uint32_t heads = min((uint32_t)kHeads, a.G - grp * kHeads);
+        const uint32_t h0 = kvh * a.G + grp * kHeads;   // first query head
+        const uint32_t my_n = p1 - p0 > warp ? (p1 - p0 - warp + kWarps - 1) / kWarps : 0;
+
+        const char *kbase = nullptr, *vbase = nullptr;
+        if constexpr (!Q8) {
+            if (a.kv.page_table) { kbase = a.kv.k_base; vbase = a.kv.v_base; }
+            else {
+                kbase = kv_seq_ptr(a.kv.k_base, a.kv.k_ptrs, a.kv.seq_stride_bytes, seq);
+                vbase = kv_seq_ptr(a.kv.v_base, a.kv.v_ptrs, a.kv.seq_stride_bytes, seq);
+            }
+        }
+        auto row_of_block = [&](uint32_t b) { return (b < sq.na ? sq.a0 + b : sq.b0 + (b - sq.na)) * kBlock; };
+        const uint32_t l_row = lane / CH % RPI, l_chunk = lane % CH;
+        // row numbers of the caches are taken relative to a base that the block's page or sequence gives
+        auto issue = [&](uint32_t i) {
+            const uint32_t r0 = row_of_block(p0 + warp + i * kWarps);
+            const uint32_t st = ring + (i % ST) * S::kStage;
+            bool have = r0 < sq.L && r0 + kBlock > sq.doc;   // some row of the block is visible: its page is the sequence's own
+            unsigned long long row0 = 0;                     // first row of the block, counted in whole cache rows
+            const char *kb = kbase, *vb = vbase;
+            if (have) {
+                if constexpr (Q8) {
+                    have = rowq_row(a.rq, seq, r0, row0);
+                    kb = reinterpret_cast<const char *>(a.rq.k_codes); vb = reinterpret_cast<const char *>(a.rq.v_codes);
+                } else if (a.kv.page_table) {
+                    have = r0 / a.kv.page_rows < a.kv.max_pages;
+                    if (have) row0 = (unsigned long long)__ldg(a.kv.page_table + (size_t)seq * a.kv.max_pages + r0 / a.kv.page_rows) * a.kv.page_rows + r0 % a.kv.page_rows;
+                } else {
+                    row0 = r0;
+                }
+            }
+            const size_t stride = (size_t)a.nkv * S::kRow;
+#pragma unroll
+            for (int k = 0; k < NI; ++k) {
+                const uint32_t r = k * RPI + l_row;
+                const bool ok = have && visible(sq, r0 + r);
+                const size_t off = ok ? (size_t)(row0 + r) * stride + (size_t)kvh * S::kRow + l_chunk * 16 : 0;
+                const uint32_t so = r * S::kRow + ((l_chunk ^ S::swz(r)) << 4);
+                cp16(st + so, kb + off, ok);
+                cp16(st + S::kTile + so, vb + off, ok);
+            }
+            if constexpr (Q8) {
+                const uint32_t r = lane & 15;
+                const bool ok = have && visible(sq, r0 + r);
+                const float *sc = lane < 16 ? a.rq.k_scales : a.rq.v_scales;
+                cp4(st + 2 * S::kTile + lane * 4, sc + (ok ? (size_t)(row0 + r) * a.nkv + kvh : 0), ok);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i) {
+            if ((uint32_t)i < my_n) issue(i);
+            cp_commit();
+        }
+
+        // ---- Q of the eight heads as T, 16-byte chunks swizzled by the head; a row-scaled cache takes a power of two out
+        //      of every head so that f16 holds it, and wants the dims in the order its byte permutes produce ----
+        for (uint32_t h = warp; h < kHeads; h += kWarps) {
+            constexpr int E = HD / 32;   // elements per lane
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = 0.f;
+            if (h < heads) {
+                const size_t o = ((size_t)seq * a.nh + h0 + h) * HD + lane * E;
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = load_as_f32(a.q, o + e, a.q_dtype);
+            }
+            float up = 1.f;
+            if constexpr (Q8) {
+                float m = 0.f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) m = fmaxf(m, fabsf(v[e]));
+                m = warp_max(m);
+                if (m > 0.f && m < INFINITY) {
+                    int ex = (int)(__float_as_uint(m) >> 23) - 127;   // 2^ex <= m < 2^(ex+1); subnormal m: -127
+                    ex = max(-126, min(126, ex));
+                    up = __uint_as_float((uint32_t)(ex + 127) << 23);
+                    const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[e] *= down;
+                }
+            }
+            if (lane == 0) sm_qs[h] = up;
+            unsigned char *rowp = sm_q + h * HD * 2;
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const uint32_t d = lane * E + e;
+                uint32_t col = d;   // column (16-bit element) of dim d
+                if constexpr (Q8) col = (d & ~15u) | ((d & 12u) >> 1) | ((d & 2u) << 2);   // 4u, 4u+1 -> 2u, 2u+1; 4u+2, 4u+3 -> 8+2u, ..
+                *reinterpret_cast<uint32_t *>(rowp + (((col >> 3) ^ (h & 7)) << 4) + (col & 7) * 2) = pack<T>(v[e], v[e + 1]);
+            }
+        }
+        __syncthreads();
+        uint32_t qb[HD / 16][2];
+#pragma unroll
+        for (int c = 0; c < HD / 16; c += 2) {
+            uint32_t r4[4];
+            ldm4(r4, q_addr + rin * HD * 2 + (((2 * c + mat) ^ rin) << 4));
+            qb[c][0] = r4[0]; qb[c][1] = r4[1]; qb[c + 1][0] = r4[2]; qb[c + 1][1] = r4[3];
+        }
+        float zscale[2], slope2[2];   // heads 2t, 2t+1
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            zscale[r] = a.rule.scale * sm_qs[2 * t + r];
+            slope2[r] = a.rule.slopes && 2 * t + r < heads ? __ldg(a.rule.slopes + h0 + 2 * t + r) * kRuleLog2e : 0.f;
+        }
+
+        float oT[HD / 16][4];
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) oT[c][0] = oT[c][1] = oT[c][2] = oT[c][3] = 0.f;
+        float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};   // l: this lane's positions only
+
+        for (uint32_t i = 0; i < my_n; ++i) {
+            cp_wait<ST - 2>();
+            __syncwarp();
+            if (i + ST - 1 < my_n) issue(i + ST - 1);
+            cp_commit();
+            const uint32_t st = ring + (i % ST) * S::kStage;
+            const uint32_t r0 = row_of_block(p0 + warp + i * kWarps);
+            // ---- S^T: 16 positions x 8 heads ----
+            float sT[4] = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (Q8) {
+#pragma unroll
+                for (int c = 0; c < CH; c += 2) {
+                    uint32_t kb[4];   // (pos 0-7, chunk c), (pos 8-15, chunk c), (.., chunk c+1), (.., chunk c+1)
+                    const uint32_t ch = c + (mat >> 1), r = (mat & 1) * 8 + rin;
+                    ldm4(kb, st + r * S::kRow + ((ch ^ S::swz(r)) << 4));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t ka[4] = {codes_to_f16<0x10>(kb[2 * h]), codes_to_f16<0x10>(kb[2 * h + 1]),
+                                                codes_to_f16<0x32>(kb[2 * h]), codes_to_f16<0x32>(kb[2 * h + 1])};
+                        mma<T>(sT, ka, qb[c + h][0], qb[c + h][1]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) {
+                    uint32_t ka[4];   // (pos 0-7, chunk 2c), (pos 8-15, chunk 2c), (pos 0-7, chunk 2c+1), (pos 8-15, chunk 2c+1)
+                    const uint32_t ch = 2 * c + (mat >> 1), r = (mat & 1) * 8 + rin;
+                    ldm4(ka, st + r * S::kRow + ((ch ^ S::swz(r)) << 4));
+                    mma<T>(sT, ka, qb[c][0], qb[c][1]);
+                }
+            }
+            // ---- the rule; this lane has positions g and g + 8 of heads 2t, 2t+1.  y = z log2(e) (+ log2 vs) ----
+            float y[4], inv_vs[2] = {1.f, 1.f};
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const uint32_t row = r0 + g + 8 * p;
+                const bool ok = visible(sq, row);
+                float ks = 1.f, lvs = 0.f;
+                if constexpr (Q8) {
+                    const float *sc = reinterpret_cast<const float *>(sm_ring + warp * ST * S::kStage + (i % ST) * S::kStage + 2 * S::kTile);
+                    ks = sc[g + 8 * p];
+                    const float vs = fminf(fmaxf(sc[kBlock + g + 8 * p], kRowqScaleMin), kRowqScaleMax);
+                    lvs = __log2f(vs);
+                    inv_vs[p] = 1.0f / vs;
+                }
+                const float dist = (float)(sq.L - 1 - row);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float z = sT[2 * p + r] * ks * zscale[r];
+                    if (a.rule.cap > 0.f) z = a.rule.cap * rule_tanh_of_exp(z * a.rule.inv_cap * (2.0f * kRuleLog2e));
+                    const float v = z * kRuleLog2e - slope2[r] * dist + lvs;
+                    y[2 * p + r] = ok ? v : -INFINITY;
+                }
+            }
+            float corr[2], pw[4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float mx = fmaxf(y[r], y[2 + r]);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float m_new = fmaxf(m_run[r], mx);
+                const float m_use = m_new == -INFINITY ? 0.f : m_new;   // nothing seen yet
+                corr[r] = rule_exp2(m_run[r] - m_use);
+                m_run[r] = m_new;
+                pw[r] = rule_exp2(y[r] - m_use);
+                pw[2 + r] = rule_exp2(y[2 + r] - m_use);
+                l_run[r] = l_run[r] * corr[r] + (pw[r] * inv_vs[0] + pw[2 + r] * inv_vs[1]);
+            }
+            const uint32_t pb0 = transpose8x8(pack<T>(pw[0], pw[1])), pb1 = transpose8x8(pack<T>(pw[2], pw[3]));
+            const bool rescale = __any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f);
+            // ---- O^T = O^T * corr + V^T P^T ----
+            if (rescale) {
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) { oT[c][0] *= corr[0]; oT[c][1] *= corr[1]; oT[c][2] *= corr[0]; oT[c][3] *= corr[1]; }
+            }
+            const uint32_t sv = st + S::kTile;
+            if constexpr (Q8) {
+#pragma unroll
+                for (int c = 0; c < CH; c += 2) {
+                    uint32_t vb[4];   // (pos 0-7, chunk c), (pos 8-15, chunk c), (.., chunk c+1), (.., chunk c+1), transposed
+                    const uint32_t ch = c + (mat >> 1), r = (mat & 1) * 8 + rin;
+                    ldm4t(vb, sv + r * S::kRow + ((ch ^ S::swz(r)) << 4));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {   // rows 0-7 of the product are the even dims of the chunk, rows 8-15 the odd ones
+                        const uint32_t va[4] = {codes_to_f16<0x20>(vb[2 * h]), codes_to_f16<0x31>(vb[2 * h]),
+                                                codes_to_f16<0x20>(vb[2 * h + 1]), codes_to_f16<0x31>(vb[2 * h + 1])};
+                        mma<T>(oT[c + h], va, pb0, pb1);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) {
+                    uint32_t va[4];   // (pos 0-7, chunk 2c), (pos 0-7, chunk 2c+1), (pos 8-15, chunk 2c), (pos 8-15, chunk 2c+1), transposed
+                    const uint32_t ch = 2 * c + (mat & 1), r = (mat >> 1) * 8 + rin;
+                    ldm4t(va, sv + r * S::kRow + ((ch ^ S::swz(r)) << 4));
+                    mma<T>(oT[c], va, pb0, pb1);
+                }
+            }
+            __syncwarp();   // the stage is free for the next request
+        }
+        cp_wait<0>();
+        // ---- the warps' states meet; the merge tiles lie in the rings ----
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 4);
+            l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 8);
+            l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 16);
+        }
+        __syncthreads();
+        float *tile = reinterpret_cast<float *>(sm_ring + warp * S::kMergeTile);
+        if (g == 0) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) { sm_m[warp * kHeads + 2 * t + r] = m_run[r]; sm_l[warp * kHeads + 2 * t + r] = l_run[r]; }
+        }
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+            const uint32_t dlo = 16 * c + (Q8 ? 2 * g : g), dhi = Q8 ? dlo + 1 : dlo + 8;
+            tile[(2 * t) * S::kORow + dlo] = oT[c][0]; tile[(2 * t + 1) * S::kORow + dlo] = oT[c][1];
+            tile[(2 * t) * S::kORow + dhi] = oT[c][2]; tile[(2 * t + 1) * S::kORow + dhi] = oT[c][3];
+        }
+        __syncthreads();
+        constexpr int kRec = HD + 2;
+        const uint32_t slot = 2 * blockIdx.x + (x == x_first ? 0u : 1u);
+        float *rec = a.records + (size_t)slot * kHeads * kRec;
+        for (uint32_t e = tid; e < heads * HD; e += kThreads) {
+            const uint32_t h = e / HD, d = e % HD;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w * kHeads + h]);
+            const float mu = M == -INFINITY ? 0.f : M;
+            float o = 0.f, l = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = rule_exp2(sm_m[w * kHeads + h] - mu);
+                o += f * reinterpret_cast<const float *>(sm_ring + w * S::kMergeTile)[h * S::kORow + d];
+                l += f * sm_l[w * kHeads + h];
+            }
+            if (whole) {
+                const size_t row = (size_t)seq * a.nh + h0 + h;
+                store_from_f32(a.out, row * HD + d, a.out_dtype, l > 0.f ? o / l : 0.f);
+                if (d == 0 && a.lse) a.lse[row] = l > 0.f ? (M + log2f(l)) * kRuleLn2 : -INFINITY;
+            } else {
+                rec[h * kRec + 2 + d] = o;
+                if (d == 0) { rec[h * kRec] = M; rec[h * kRec + 1] = l; }
+            }
+        }
+        if (!whole) {
+            // ---- the last CTA to arrive joins the records of this (sequence, kv head, group) ----
+            const uint32_t c0 = u0 / share, c1 = (u1 - 1) / share, nrec = c1 - c0 + 1;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) *sm_flag = atomicAdd(a.counters + (size_t)seq * U + unit, 1u);
+            __syncthreads();
+            if (*sm_flag == nrec - 1) {
+                __threadfence();
+                if (tid == 0) a.counters[(size_t)seq * U + unit] = 0;
+                // share c0 wrote the piece as its last one (slot 1) unless the piece began with the share
+                const uint32_t slot0 = 2 * c0 + (u0 == c0 * share ? 0u : 1u);
+                auto record = [&](uint32_t k) { return a.records + (size_t)(k ? 2 * (c0 + k) : slot0) * kHeads * kRec; };
+                for (uint32_t e = tid; e < heads * HD; e += kThreads) {
+                    const uint32_t h = e / HD, d = e % HD;
+                    float M = -INFINITY, o = 0.f, l = 0.f;
+                    for (uint32_t k0 = 0; k0 < nrec; k0 += 8) {
+                        float rm[8], rl[8], ro[8];
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k) {
+                            rm[k] = -INFINITY; rl[k] = 0.f; ro[k] = 0.f;
+                            if (k0 + k < nrec) {
+                                const float *r = record(k0 + k) + h * kRec;
+                                rm[k] = __ldcg(r); rl[k] = __ldcg(r + 1); ro[k] = __ldcg(r + 2 + d);
+                            }
+                        }
+                        float mx = M;
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k) mx = fmaxf(mx, rm[k]);
+                        const float mu = mx == -INFINITY ? 0.f : mx, f0 = rule_exp2(M - mu);
+                        o *= f0; l *= f0;
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k) {
+                            const float f = rule_exp2(rm[k] - mu);
+                            o += f * ro[k]; l += f * rl[k];
+                        }
+                        M = mx;
+                    }
+                    const size_t row = (size_t)seq * a.nh + h0 + h;
+                    store_from_f32(a.out, row * HD + d, a.out_dtype, l > 0.f ? o / l : 0.f);
+                    if (d == 0 && a.lse) a.lse[row] = l > 0.f ? (M + log2f(l)) * kRuleLn2 : -INFINITY;
+                }
+            }
+        }
+        __syncthreads();   // the rings and the statistics are free for the next piece
+        x = u0 + p1;
+        if (x >= u1 && unit == U - 1) { base = u1; ++seq; }
+    }
+}
+
+static uint32_t head_groups(const shady_decode_params *p) { return (p->num_q_heads / p->num_kv_heads + kHeads - 1) / kHeads; }
+static int check(shady_ctx *ctx, const shady_decode_params *p) {
+    SHADY_REQUIRE(ctx, p, SHADY_ERR_BAD_ARG, "decode_rule: null parameters");
+    SHADY_REQUIRE(ctx, p->num_kv_heads && p->num_q_heads && p->num_seqs, SHADY_ERR_BAD_ARG, "decode_rule: zero-sized problem");
+    SHADY_REQUIRE(ctx, p->num_q_heads % p->num_kv_heads == 0 && (!p->heads_per_kv || p->heads_per_kv == p->num_q_heads / p->num_kv_heads),
+                  SHADY_ERR_BAD_ARG, "decode_rule: num_q_heads must be num_kv_heads * heads_per_kv");
+    SHADY_REQUIRE(ctx, p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256, SHADY_ERR_UNSUPPORTED,
+                  "decode_rule: head_dim must be 64, 128 or 256");
+    SHADY_REQUIRE(ctx, p->num_splits == 0, SHADY_ERR_UNSUPPORTED, "decode_rule: num_splits must be 0 (shares are worked out on the device)");
+    SHADY_REQUIRE(ctx, p->q_dtype <= SHADY_BF16 && p->out_dtype <= SHADY_BF16, SHADY_ERR_BAD_ARG, "decode_rule: bad dtype");
+    return SHADY_OK;
+}
+constexpr uint32_t kMaxCtasPerSm = 3;
+static size_t counter_bytes(const shady_decode_params *p) {
+    return ((size_t)p->num_seqs * p->num_kv_heads * head_groups(p) * 4 + 255) & ~(size_t)255;
+}
+static size_t workspace_bytes(const shady_ctx *ctx, const shady_decode_params *p) {
+    return counter_bytes(p) + (size_t)2 * ctx->num_sms * kMaxCtasPerSm * kHeads * (p->head_dim + 2) * 4;
+}
+
+template <typename T, int HD, bool Q8> static int launch(shady_ctx *ctx, const Args &a) {
+    using S = Smem<HD, Q8>;
+    static_assert(S::kCtas <= (int)kMaxCtasPerSm && S::kCtas * (S::kTotal + 1024) <= 228 * 1024, "resident CTAs");
+    auto kern = decode_rule_kernel<T, HD, Q8>;
+    SHADY_CUDA_OK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal));
+    kern<<<ctx->num_sms * S::kCtas, kThreads, S::kTotal, ctx->stream>>>(a);
+    ctx->launches++;
+    SHADY_CUDA_OK(ctx, cudaGetLastError());
+    return SHADY_OK;
+}
+
+}  // namespace dr
+
+int decode_rule_workspace_size(shady_ctx *ctx, const shady_decode_params *p, size_t *bytes) {
+    if (const int st = dr::check(ctx, p)) return st;
+    SHADY_REQUIRE(ctx, bytes, SHADY_ERR_BAD_ARG, "decode_rule: null argument");
+    *bytes = dr::workspace_bytes(ctx, p);
+    return SHADY_OK;
+}
+int decode_rule_workspace_init(shady_ctx *ctx, const shady_decode_params *p, void *d_ws, size_t ws_bytes) {
+    if (const int st = dr::check(ctx, p)) return st;
+    SHADY_REQUIRE(ctx, d_ws && ws_bytes >= dr::workspace_bytes(ctx, p), SHADY_ERR_WORKSPACE, "decode_rule: workspace missing or too small");
+    SHADY_CUDA_OK(ctx, cudaMemsetAsync(d_ws, 0, dr::counter_bytes(p), ctx->stream));
+    return SHADY_OK;
+}
+
+int launch_decode_rule(shady_ctx *ctx, const shady_decode_params *p, const shady_score_rule *rule, const void *d_q,
+                       const shady_kv_cache *cache, const shady_rowq_cache *rowq, const uint32_t *d_seq_lens, void *d_out, float *d_lse,
+                       void *d_ws, size_t ws_bytes) {
+    if (const int st = dr::check(ctx, p)) return st;
+    SHADY_REQUIRE(ctx, d_q && d_seq_lens && d_out, SHADY_ERR_BAD_ARG, "decode_rule: null argument");
+    SHADY_REQUIRE(ctx, !cache != !rowq, SHADY_ERR_BAD_ARG, "decode_rule: exactly one of a 16-bit and a row-scaled cache");
+    SHADY_REQUIRE(ctx, ((uintptr_t)d_q & 15) == 0 && ((uintptr_t)d_out & 15) == 0, SHADY_ERR_BAD_ARG, "decode_rule: q and out must be 16-byte aligned");
+    dr::Args a{};
+    if (const int st = fill_rule(ctx, rule, p->head_dim, "decode_rule", &a.rule)) return st;
+    if (cache) {
+        SHADY_REQUIRE(ctx, cache->dtype == SHADY_F16 || cache->dtype == SHADY_BF16, SHADY_ERR_UNSUPPORTED, "decode_rule: the cache must be f16 or bf16 (or row-scaled)");
+        SHADY_REQUIRE(ctx, p->q_dtype == SHADY_F32 || p->q_dtype == cache->dtype, SHADY_ERR_UNSUPPORTED, "decode_rule: q must be f32 or the cache dtype");
+        if (const int st = fill_kv_addr(ctx, cache, p->num_kv_heads, p->head_dim, "decode_rule", &a.kv)) return st;
+        SHADY_REQUIRE(ctx, ((uintptr_t)cache->d_k_base & 15) == 0 && ((uintptr_t)cache->d_v_base & 15) == 0 && a.kv.seq_stride_bytes % 16 == 0,
+                      SHADY_ERR_BAD_ARG, "decode_rule: cache rows must be 16-byte aligned");
+    } else {
+        if (const int st = fill_rowq_addr(ctx, rowq, "decode_rule", &a.rq)) return st;
+    }
+    SHADY_REQUIRE(ctx, d_ws && ((uintptr_t)d_ws & 15) == 0 && ws_bytes >= dr::workspace_bytes(ctx, p), SHADY_ERR_WORKSPACE,
+                  "decode_rule: workspace missing, unaligned or too small");
+    a.q = d_q; a.out = d_out; a.lse = d_lse; a.lens = d_seq_lens;
+    a.counters = reinterpret_cast<uint32_t *>(d_ws);
+    a.records = reinterpret_cast<float *>(reinterpret_cast<char *>(d_ws) + dr::counter_bytes(p));
+    a.num_seqs = p->num_seqs; a.nkv = p->num_kv_heads; a.nh = p->num_q_heads; a.G = a.nh / a.nkv; a.groups = dr::head_groups(p);
+    a.q_dtype = p->q_dtype; a.out_dtype = p->out_dtype;
+    auto by_dim = [&](auto t, auto q8) {
+        using T = decltype(t);
+        constexpr bool Q8 = decltype(q8)::value;
+        if (p->head_dim == 64) return dr::launch<T, 64, Q8>(ctx, a);
+        if (p->head_dim == 128) return dr::launch<T, 128, Q8>(ctx, a);
+        return dr::launch<T, 256, Q8>(ctx, a);
+    };
+    if (rowq) return by_dim(__half{}, std::true_type{});
+    if (cache->dtype == SHADY_F16) return by_dim(__half{}, std::false_type{});
+    return by_dim(__nv_bfloat16{}, std::false_type{});
+}
+
+}  // namespace shady

@@ -1,0 +1,60 @@
+// The row-scaled 8-bit KV cache: device-side addressing and the code <-> value arithmetic shared by the kernels that
+// write it (append), read it back, and attend over it.
+#pragma once
+#include "common.cuh"
+
+namespace shady {
+
+constexpr float kRowqCodeMax = 127.0f;
+constexpr float kRowqScaleMin = 8.673617379884035e-19f;   // 2^-60
+constexpr float kRowqScaleMax = 1.152921504606847e18f;    // 2^60
+
+struct RowqAddr {
+    unsigned char *k_codes, *v_codes;
+    float *k_scales, *v_scales;
+    unsigned long long seq_rows;
+    const uint32_t *page_table;
+    uint32_t page_rows, max_pages, num_pages;
+};
+
+// Row of `pos` of sequence s in the code and scale arrays; false if it lies behind the sequence's cache, or on a page
+// that the pool does not have.
+__device__ __forceinline__ bool rowq_row(const RowqAddr &c, uint32_t s, uint32_t pos, unsigned long long &row) {
+    if (c.page_table) {
+        const uint32_t pi = pos / c.page_rows;
+        if (pi >= c.max_pages) return false;
+        const uint32_t pg = __ldg(c.page_table + (size_t)s * c.max_pages + pi);
+        if (c.num_pages && pg >= c.num_pages) return false;
+        row = (unsigned long long)pg * c.page_rows + pos % c.page_rows;
+        return true;
+    }
+    row = (unsigned long long)s * c.seq_rows + pos;
+    return pos < c.seq_rows;
+}
+
+// scale of a row from its largest magnitude (fmaxf has dropped NaNs on the way; an infinity ends at the upper bound)
+__device__ __forceinline__ float rowq_scale(float amax) { return fminf(fmaxf(amax / kRowqCodeMax, kRowqScaleMin), kRowqScaleMax); }
+// x / scale to the nearest code, -127 .. 127; inv = 1 / scale.  cvt.rni turns a NaN into 0 and saturates infinities.
+__device__ __forceinline__ int rowq_code(float x, float inv) { return max(-127, min(127, __float2int_rn(x * inv))); }
+
+// Checks a caller's description and turns it into the device-side form (append_rowq.cu).
+int fill_rowq_addr(shady_ctx *ctx, const shady_rowq_cache *cache, const char *who, RowqAddr *out);
+
+// The sequence that owns packed item `at` of a batch whose starts[num_seqs + 1] do not fall: the s with
+// starts[s] <= at < starts[s + 1].  The warp narrows the range 32-fold per step; `at` is warp-uniform and lies
+// below starts[num_seqs].
+__device__ __forceinline__ uint32_t warp_find_seq(const uint32_t *starts, uint32_t num_seqs, uint32_t at, uint32_t lane) {
+    uint32_t lo = 0, n = num_seqs;   // the answer is the last s in [lo, lo + n) with starts[s] <= at
+    while (n > 1) {
+        const uint32_t step = (n + 31) / 32;
+        const uint32_t i = lane * step;
+        const bool le = i < n && __ldg(starts + lo + i) <= at;
+        const uint32_t votes = __ballot_sync(0xffffffffu, le);   // lane 0 votes yes unless starts[lo] > at, which the caller rules out
+        const uint32_t k = votes ? 31 - __clz(votes) : 0;
+        lo += k * step;
+        n = min(step, n - k * step);
+    }
+    return lo;
+}
+
+}  // namespace shady

@@ -1,0 +1,38 @@
+// Score rules of the rule attention kernels: what a query sees, and what happens to its scores (shady_score_rule).
+#pragma once
+#include <math.h>
+
+#include "common.cuh"
+
+namespace shady {
+
+constexpr float kRuleLog2e = 1.4426950408889634f;
+constexpr float kRuleLn2 = 0.6931471805599453f;
+
+struct RuleArgs {
+    float scale;          // z = q.k * scale
+    float cap, inv_cap;   // cap > 0: z = cap * tanh(z * inv_cap)
+    uint32_t window;      // 0 = none
+    const float *slopes;
+    const uint32_t *prefix, *doc;
+};
+
+// Checks a caller's rule and turns it into the device-side form (decode_rule.cu).
+int fill_rule(shady_ctx *ctx, const shady_score_rule *rule, uint32_t head_dim, const char *who, RuleArgs *out);
+
+__device__ __forceinline__ float rule_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rule_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// tanh(z) = 1 - 2 / (1 + e^(2z)), with z2 = 2 z log2(e).  The absolute error is a few 2^-24 everywhere (near 0 the
+// two halves cancel, but a score needs cap * tanh to an absolute error, not a relative one); tanh.approx is 2^-11 off,
+// which a cap of 50 turns into 2 % of a weight.
+__device__ __forceinline__ float rule_tanh_of_exp(float z2) { return 1.0f - 2.0f * rule_rcp(1.0f + rule_exp2(z2)); }
+
+}  // namespace shady

@@ -8,7 +8,8 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import _lib
-from ._lib import BF16, F8E4M3, F16, F32, AppendParams, DecodeParams, GptqWeight, KvCache, PrefillParams
+from ._lib import (BF16, F8E4M3, F16, F32, AppendParams, DecodeParams, GptqWeight, KvCache, PrefillParams, RowqCache,
+                   ScoreRuleC)
 from .gpu import GpuContext, _addr
 
 _TORCH_DTYPES = None
@@ -284,6 +285,120 @@ def qkv_proj_append(gpu: GpuContext, *, wq: GptqMatrix, wk: GptqMatrix, wv: Gptq
     gpu._check(gpu._L.shady_qkv_proj_append(gpu.handle, C.byref(p), C.byref(cq), C.byref(ck), C.byref(cv), _addr(x),
                                             _addr(q_out), _addr(q_gate) or None, C.byref(c), _addr(qk_norm_bf16) or None,
                                             _addr(pos_start), _addr(pos_h) or None, _addr(pos_w) or None))
+
+
+@dataclass
+class RowqCacheView:
+    """A row-scaled 8-bit cache (``shady_rowq_cache``): codes ``[rows][nkv][hd]`` u8 and scales ``[rows][nkv]`` f32 for K
+    and V, either one allocation with ``seq_rows`` rows per sequence or pools of pages behind a page table."""
+
+    k_codes: object
+    v_codes: object
+    k_scales: object
+    v_scales: object
+    seq_rows: int = 0
+    page_table: object = None    # device u32 [num_seqs][max_pages_per_seq]
+    page_rows: int = 0
+    max_pages_per_seq: int = 0
+    num_pages: int = 0           # pages of the pools; 0: table entries are not checked
+
+    def c_struct(self) -> RowqCache:
+        return RowqCache(_addr(self.k_codes) or None, _addr(self.v_codes) or None, _addr(self.k_scales) or None,
+                         _addr(self.v_scales) or None, self.seq_rows, _addr(self.page_table) or None, self.page_rows,
+                         self.max_pages_per_seq, self.num_pages, 0)
+
+
+@dataclass
+class ScoreRule:
+    """What a query sees and what happens to its scores (``shady_score_rule``).  ``scale`` 0 means 1/sqrt(head_dim),
+    ``cap`` and ``window`` 0 mean none; the arrays are device buffers."""
+
+    scale: float = 0.0
+    cap: float = 0.0
+    slopes: object = None        # f32 [num_q_heads]
+    window: int = 0
+    prefix_lens: object = None   # u32 [num_seqs]
+    doc_start: object = None     # u32: decode [num_seqs], prefill [tokens]
+
+    def c_struct(self) -> ScoreRuleC:
+        return ScoreRuleC(self.scale, self.cap, self.window, 0, _addr(self.slopes) or None, _addr(self.prefix_lens) or None,
+                          _addr(self.doc_start) or None)
+
+
+def kv_append_rowq(gpu: GpuContext, *, q_proj_full, k_proj, v_proj, q_out, q_gate, cache: RowqCacheView, pos_start,
+                   num_heads: int, num_kv_heads: int, head_dim: int, rope_theta: float, rotary_dim: int,
+                   interleaved: bool = True, eps: float = 1e-6, qk_norm_bf16=None, num_seqs: int = 1,
+                   tokens_per_seq: int = 1, in_dtype: int = F32, q_dtype: int = F32, has_gate: bool = True, k_out=None,
+                   v_out=None, pos_h=None, pos_w=None, s1_limit: int | None = None, s2_limit: int | None = None,
+                   tok_start=None, total_tokens: int | None = None) -> None:
+    """``kv_append_rope`` into a row-scaled cache; ``k_out`` / ``v_out`` receive the rows as the cache holds them.  With
+    ``tok_start`` (device u32 [num_seqs + 1]) the tokens are packed and ``total_tokens`` bounds their number."""
+    p = AppendParams(num_heads, num_kv_heads, head_dim, eps, rope_theta, rotary_dim,
+                     rotary_dim // 2 if s1_limit is None else s1_limit,
+                     rotary_dim // 2 if s2_limit is None else s2_limit, int(interleaved), num_seqs,
+                     tokens_per_seq, in_dtype, q_dtype, int(has_gate), 0, 0)
+    c = cache.c_struct()
+    n = num_seqs * tokens_per_seq if total_tokens is None else total_tokens
+    gpu._check(gpu._L.shady_kv_append_rowq(gpu.handle, C.byref(p), _addr(q_proj_full), _addr(k_proj), _addr(v_proj),
+                                           _addr(q_out), _addr(q_gate) or None, _addr(k_out) or None, _addr(v_out) or None,
+                                           C.byref(c), _addr(qk_norm_bf16) or None, _addr(pos_start), _addr(pos_h) or None,
+                                           _addr(pos_w) or None, _addr(tok_start) or None, n))
+
+
+def kv_read_rowq(gpu: GpuContext, *, cache: RowqCacheView, out_start, total_rows: int, num_seqs: int, num_kv_heads: int,
+                 head_dim: int, k_out=None, v_out=None, row_start=None, out_dtype: int = BF16) -> None:
+    """Listed row ranges of a row-scaled cache as packed rows: ``out_start`` (device u32 [num_seqs + 1]) says where each
+    sequence's rows go, ``row_start`` (device u32 [num_seqs], or None for 0) where they begin in its cache."""
+    c = cache.c_struct()
+    gpu._check(gpu._L.shady_kv_read_rowq(gpu.handle, C.byref(c), num_kv_heads, head_dim, num_seqs, _addr(row_start) or None,
+                                         _addr(out_start), total_rows, _addr(k_out) or None, _addr(v_out) or None, out_dtype))
+
+
+def _rule_params(head_dim: int, num_kv_heads: int, num_q_heads: int, num_seqs: int, q_dtype: int = F32,
+                 out_dtype: int = F32) -> DecodeParams:
+    return DecodeParams(head_dim, num_kv_heads, num_q_heads, num_q_heads // num_kv_heads if num_kv_heads else 0, 0, num_seqs,
+                        q_dtype, out_dtype)
+
+
+def decode_rule_workspace_size(gpu: GpuContext, *, head_dim: int, num_kv_heads: int, num_q_heads: int, num_seqs: int) -> int:
+    p = _rule_params(head_dim, num_kv_heads, num_q_heads, num_seqs)
+    n = C.c_size_t()
+    gpu._check(gpu._L.shady_decode_rule_workspace_size(gpu.handle, C.byref(p), C.byref(n)))
+    return n.value
+
+
+def decode_rule_workspace_init(gpu: GpuContext, workspace, workspace_bytes: int, *, head_dim: int, num_kv_heads: int,
+                               num_q_heads: int, num_seqs: int) -> None:
+    """Zero the arrival counters at the head of a freshly allocated workspace (once)."""
+    p = _rule_params(head_dim, num_kv_heads, num_q_heads, num_seqs)
+    gpu._check(gpu._L.shady_decode_rule_workspace_init(gpu.handle, C.byref(p), _addr(workspace) or None, workspace_bytes))
+
+
+def attn_decode_rule(gpu: GpuContext, *, q, cache: KvCacheView | RowqCacheView, seq_lens, out, head_dim: int,
+                     num_kv_heads: int, num_q_heads: int, num_seqs: int = 1, rule: ScoreRule | None = None,
+                     q_dtype: int = F32, out_dtype: int = F32, lse=None, workspace=None, workspace_bytes: int = 0) -> None:
+    """Attention of one new token per sequence under a score rule, over a 16-bit or a row-scaled cache.  The lengths are
+    read on the device only."""
+    p = _rule_params(head_dim, num_kv_heads, num_q_heads, num_seqs, q_dtype, out_dtype)
+    c = cache.c_struct()
+    r = C.byref(rule.c_struct()) if rule is not None else None
+    kv, rowq = (None, C.byref(c)) if isinstance(cache, RowqCacheView) else (C.byref(c), None)
+    gpu._check(gpu._L.shady_attn_decode_rule(gpu.handle, C.byref(p), r, _addr(q), kv, rowq, _addr(seq_lens), _addr(out),
+                                             _addr(lse) or None, _addr(workspace) or None, workspace_bytes))
+
+
+def attn_prefill_rule(gpu: GpuContext, *, q, cache: KvCacheView, cache_rows: int, q_starts, kv_lens, out, head_dim: int,
+                      num_kv_heads: int, num_q_heads: int, num_seqs: int, total_q: int, dtype: int = BF16, kv_starts=None,
+                      rule: ScoreRule | None = None, lse=None) -> None:
+    """Attention of packed tokens (``q_starts``: device u32 [num_seqs + 1]) over rows that are in the cache, under a score
+    rule.  ``kv_starts`` (device u32 [num_seqs]): where each sequence's rows begin among ``cache_rows`` packed rows; None
+    for ``cache.seq_stride`` or a page table.  ``kv_lens`` (device u32 [num_seqs]) counts the tokens' own rows."""
+    p = PrefillParams(head_dim, num_kv_heads, num_q_heads, num_seqs, 0, dtype)
+    c = cache.c_struct()
+    r = C.byref(rule.c_struct()) if rule is not None else None
+    gpu._check(gpu._L.shady_attn_prefill_rule(gpu.handle, C.byref(p), r, _addr(q), C.byref(c), cache_rows, _addr(q_starts),
+                                              total_q, _addr(kv_starts) or None, _addr(kv_lens), _addr(out),
+                                              _addr(lse) or None))
 
 
 def sigmoid_mul(gpu: GpuContext, x, gate, n: int) -> None:
