@@ -1,68 +1,639 @@
-// Attention of many tokens per sequence under a score rule, over rows that are in a 16-bit cache.
+// Attention of many tokens per sequence under a score rule, over rows that are in a 16-bit cache, on the 5th-generation
+// tensor cores (tcgen05 + TMEM) fed by TMA.
 //
 // Token t of a sequence with T tokens and L rows is the query at position i = L - T + t; z_j, out and lse are those of
 // decode_rule.cu, over the rows j that the rule lets position i see (shady_score_rule).
+//
+// What bounds it: 4 hd operations per (query head, visible row) on the tensor pipe against one exponential (three with a
+// tanh cap, of which a pair of elements shares one reciprocal) on the special function unit, which runs 16 per clock
+// and SM: at head_dim 128 a 128 x 128 tile owes the tensor pipe 1,024 clocks, the exponentials 1,024, a cap 1,536 more.
+//
+//   * The query heads of a kv head share a row tile: row r of a tile is token r / G, head r % G (G heads per kv head,
+//     128 / G whole tokens per tile).  K and V are then fetched once for all of them, a chunk of a few tokens fills a
+//     tile, and the causal edge of a tile is 128 / G tokens wide.  A TMA box of (64 dims, G heads, 128 / G tokens) lays Q
+//     out like that by itself.
+//   * An item is two row tiles (head_dim 256: one, S and O of two would need 768 TMEM columns) of one (sequence, kv head).
+//     One warp finds the items: it walks the sequences' lengths in device memory, latest tokens first, takes every
+//     gridDim.x-th item in serpentine order and works out which K/V tiles a row of it can see (window, documents, prefix),
+//     so nothing is planned on the host and a captured launch serves other lengths.  The other warps take items from a
+//     two-deep ring in shared memory.
+//   * K and V tiles come through rings of their own (a K slot is free once its scores are computed); rows past a
+//     sequence's end may hold anything, so a warp of its own clears them in the V tile (0 * NaN) before the MMA.
+//   * Softmax, one thread per row: the tile's scores are taken to registers whole, transformed, masked by four 32-bit
+//     words that interval arithmetic gives (skipped by a warp whose rows see the whole tile), and P goes back over S as
+//     the A operand of the second MMA.  O is only rescaled when a row's maximum grew by more than 2^8.
+// Every wait is bounded (see shady_ctx_set_wait_limits).
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "rowq.cuh"
 #include "rule.cuh"
+#include "tc.cuh"
 
 namespace shady {
 namespace pr {
 
 struct Args {
     RuleArgs rule;
-    const void *q;
+    StatusRef status;
+    uint32_t wait_mbar;
     void *out;
     float *lse;
-    const char *k_base, *v_base;
     const uint32_t *page_table;
-    uint32_t page_rows, max_pages;
-    unsigned long long seq_rows, cache_rows;
+    uint32_t page_rows, max_pages, box_rows;
+    unsigned long long seq_rows;
     const uint32_t *q_starts, *kv_starts, *kv_lens;
     uint32_t num_seqs, total_q, nkv, nh, G;
 };
 
-// One warp per (token, head), the rows one after the other, running maximum and sum in f32.
-template <typename T, int HD>
-__global__ void __launch_bounds__(128) prefill_rule_kernel(const __grid_constant__ Args a) {
-    constexpr int E = HD / 32;
-    const uint32_t lane = threadIdx.x & 31;
-    const unsigned long long unit = (unsigned long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const uint32_t tok = (uint32_t)(unit / a.nh), h = (uint32_t)(unit % a.nh);
-    if (tok >= min(a.total_q, __ldg(a.q_starts + a.num_seqs))) return;
-    const uint32_t seq = warp_find_seq(a.q_starts, a.num_seqs, tok, lane);
-    const uint32_t L = __ldg(a.kv_lens + seq), q1 = __ldg(a.q_starts + seq + 1);
-    const long long pos = (long long)L - (q1 - tok);
-    const uint32_t doc = a.rule.doc ? __ldg(a.rule.doc + tok) : 0u, pre = a.rule.prefix ? min(__ldg(a.rule.prefix + seq), L) : 0u;
-    const long long wlo = a.rule.window ? max((long long)doc, pos + 1 - (long long)a.rule.window) : (long long)doc;
-    const float slope = a.rule.slopes ? __ldg(a.rule.slopes + h) : 0.f;
-    float q[E], o[E], m = -INFINITY, l = 0.f;
-    const size_t qo = ((size_t)tok * a.nh + h) * HD + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) { q[e] = to_f32<T>(reinterpret_cast<const T *>(a.q)[qo + e]); o[e] = 0.f; }
-    for (uint32_t j = doc; pos >= 0 && j < L; ++j) {
-        if (!((long long)j <= pos && (long long)j >= wlo) && j >= pre) continue;
-        unsigned long long row;
-        if (a.page_table) row = (unsigned long long)__ldg(a.page_table + (size_t)seq * a.max_pages + j / a.page_rows) * a.page_rows + j % a.page_rows;
-        else row = (a.kv_starts ? __ldg(a.kv_starts + seq) : seq * a.seq_rows) + j;
-        if (row >= a.cache_rows) continue;
-        const size_t off = (row * a.nkv + h / a.G) * HD + lane * E;
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += q[e] * to_f32<T>(reinterpret_cast<const T *>(a.k_base)[off + e]);
-        float z = warp_sum(s) * a.rule.scale;
-        if (a.rule.cap > 0.f) z = a.rule.cap * rule_tanh_of_exp(z * a.rule.inv_cap * (2.0f * kRuleLog2e));
-        z -= slope * fabsf((float)(pos - (long long)j));
-        const float mn = fmaxf(m, z), c = expf(m - mn), p = expf(z - mn);
-        l = l * c + p;
-        m = mn;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * c + p * to_f32<T>(reinterpret_cast<const T *>(a.v_base)[off + e]);
+template <int HD> struct Cfg {
+    static constexpr uint32_t kNT = HD == 128 ? 2 : 1;          // row tiles of an item
+    static constexpr uint32_t kN = HD == 128 ? 128 : 64;        // K/V rows of a tile
+    static constexpr uint32_t kNS = HD == 128 ? 1 : 3;          // score buffers of a row tile
+    static constexpr uint32_t kAhead = kNS - 1;                 // score tiles issued ahead of the PV of a tile
+    static constexpr uint32_t kSlabs = HD / 64;                 // 64-element (128-byte) slabs of a row
+    static constexpr uint32_t kKvSlab = kN * 128, kKvTile = kSlabs * kKvSlab;
+    static constexpr uint32_t kQSlab = 128 * 128, kQTile = kSlabs * kQSlab;
+    static constexpr uint32_t kKS = 3, kVS = 2;                 // slots of the K and V rings
+    static constexpr uint32_t kSmemK = kNT * kQTile, kSmemV = kSmemK + kKS * kKvTile, kSmemMisc = kSmemV + kVS * kKvTile;
+    static constexpr uint32_t kSmem = kSmemMisc + 512 + 1024;   // barriers, item ring; slack for 1024-byte alignment
+    static constexpr uint32_t kColO = 256;                      // TMEM: scores below, O_q at 256 + 128 q
+    static constexpr uint32_t kThreads = kNT * 128 + 128;
+    static_assert(kSmem <= 232448, "Q and the rings must fit in 227 KB");
+    static_assert(kNT * kNS * kN <= kColO && kColO + kNT * HD <= 512, "TMEM columns");
+};
+enum { B_IFULL = 0, B_IEMPTY = 2, B_QFULL = 4, B_QEMPTY = 6, B_KFULL = 8, B_KEMPTY = 11, B_VFULL = 14, B_VEMPTY = 16, B_VFIX = 18,
+       B_SFULL = 19, B_PFULL = 22, B_OFULL = 25, B_VREQ = 27, B_PVDONE = 28, B_COUNT = 31 };
+constexpr uint32_t kItemOff = 8 * B_COUNT + 16;   // two item descriptors of 16 words behind the barriers, the TMEM slot and the abort word
+static_assert(kItemOff + 2 * 64 <= 512, "barriers and item ring");
+// The warps of head_dim 128 start with 168 registers each (384 threads); the softmax warpgroups hold a whole row of scores.
+constexpr uint32_t kRegsSoftmax = 216, kRegsOther = 72, kRegsLaunch = 168;
+static_assert(2 * kRegsSoftmax + kRegsOther <= 3 * kRegsLaunch, "setmaxnreg can only hand out what the block was launched with");
+
+struct Item {
+    uint32_t valid, seq, kvh, tok0, ntok;
+    int32_t pos0;                  // position of the first token (negative: in front of the first row)
+    uint32_t L, row0;              // rows of the sequence; its first row in a packed cache
+    uint32_t a0, na, b0, n;        // K/V tiles: a0 .. a0+na-1, then b0 ..; n in all
+    uint32_t pre;                  // prefix rows
+    __device__ __forceinline__ uint32_t tile(uint32_t j) const { return j < na ? a0 + j : b0 + (j - na); }
+};
+__device__ __forceinline__ Item item_read(const volatile uint32_t *w) {
+    Item it;
+    it.valid = w[0]; it.seq = w[1]; it.kvh = w[2]; it.tok0 = w[3]; it.ntok = w[4]; it.pos0 = (int32_t)w[5]; it.L = w[6]; it.row0 = w[7];
+    it.a0 = w[8]; it.na = w[9]; it.b0 = w[10]; it.n = w[11]; it.pre = w[12];
+    return it;
+}
+// bits [lo, hi) of a 32-bit word, any lo and hi
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+    lo = max(lo, 0); hi = min(hi, 32);
+    if (lo >= hi) return 0u;
+    return (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+
+// MODE 0: scale only, 1: tanh cap, 2: distance bias, with or without a cap
+template <typename T, int HD, int MODE>
+__global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
+prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ Args a) {
+    using C = Cfg<HD>;
+    constexpr uint32_t NT = C::kNT, N = C::kN, NS = C::kNS;
+    constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;   // swizzled tiles need 1024-byte alignment
+    unsigned char *smem = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t bar0 = smem_base + C::kSmemMisc;
+    auto bar = [&](uint32_t i) { return bar0 + 8u * i; };
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem + C::kSmemMisc + 8 * B_COUNT);
+    volatile uint32_t *abort_word = tmem_slot + 1;
+    volatile uint32_t *items = reinterpret_cast<volatile uint32_t *>(smem + C::kSmemMisc + kItemOff);
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (gave_up(a.status)) return;
+    const WaitCtx wc{abort_word, a.status, a.wait_mbar};
+    constexpr uint32_t kWProd = 4 * NT, kWMma = kWProd + 1, kWSched = kWProd + 2, kWFix = kWProd + 3;
+    const uint32_t TPT = 128u / a.G, R = TPT * a.G, TPI = NT * TPT;   // tokens and rows of a tile, tokens of an item
+
+    if (warp == kWProd && lane == 0) {
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(bar(B_IFULL + i), 1);
+            mbar_init(bar(B_IEMPTY + i), 3 + 4 * NT);   // producer, issuer, V clearing warp, softmax warps
+            mbar_init(bar(B_QFULL + i), 1); mbar_init(bar(B_QEMPTY + i), 1); mbar_init(bar(B_OFULL + i), 1);
+        }
+        for (uint32_t i = 0; i < C::kKS; ++i) { mbar_init(bar(B_KFULL + i), 1); mbar_init(bar(B_KEMPTY + i), 1); }
+        for (uint32_t i = 0; i < C::kVS; ++i) { mbar_init(bar(B_VFULL + i), 1); mbar_init(bar(B_VEMPTY + i), 1); }
+        for (uint32_t i = 0; i < 3; ++i) { mbar_init(bar(B_SFULL + i), 1); mbar_init(bar(B_PFULL + i), 128); mbar_init(bar(B_PVDONE + i), 1); }
+        mbar_init(bar(B_VREQ), 1); mbar_init(bar(B_VFIX), 1);
+        *abort_word = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == kWMma) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    // the next item of the ring; false when the list has ended or a wait gave up.  A role of one thread and
+    // one of a whole warp differ in who says that the slot has been read.
+    auto take_item = [&](uint32_t ic, Item &it, auto whole_warp, int code) {
+        if (!mbar_wait(bar(B_IFULL + (ic & 1)), (ic >> 1) & 1, wc, code)) return false;
+        it = item_read(items + 16 * (ic & 1));
+        if constexpr (decltype(whole_warp)::value) __syncwarp();
+        if (!decltype(whole_warp)::value || lane == 0) mbar_arrive(bar(B_IEMPTY + (ic & 1)));
+        return it.valid != 0;
+    };
+    constexpr std::true_type kWarpRole{};
+    constexpr std::false_type kThreadRole{};
+
+    if (warp >= kWProd) {
+    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == kWSched) {
+        // =============================== items ===============================
+        uint32_t chunk = 0, base = 0, upto = 0, mine = 0, all = 0, ic = 0;   // 32 sequences at a time, one per lane
+        uint32_t qs = 0, T_s = 0;
+        auto load_chunk = [&]() {
+            const uint32_t s = chunk + lane;
+            qs = T_s = 0;
+            if (s < a.num_seqs) {
+                qs = min(__ldg(a.q_starts + s), a.total_q);
+                T_s = max(min(__ldg(a.q_starts + s + 1), a.total_q), qs) - qs;
+            }
+            mine = (T_s + TPI - 1) / TPI * a.nkv;
+            upto = mine;
 #pragma unroll
-    for (int e = 0; e < E; ++e) reinterpret_cast<T *>(a.out)[qo + e] = from_f32<T>(l > 0.f ? o[e] / l : 0.f);
-    if (lane == 0 && a.lse) a.lse[(size_t)tok * a.nh + h] = l > 0.f ? m + logf(l) : -INFINITY;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= (uint32_t)o) upto += v;
+            }
+            all = __shfl_sync(0xffffffffu, upto, 31);
+        };
+        load_chunk();
+        bool ok = true, more = true;
+        for (uint32_t rnd = 0; more && ok; ++rnd, ++ic) {
+            const uint32_t w = rnd * gridDim.x + ((rnd & 1u) ? gridDim.x - 1u - blockIdx.x : blockIdx.x);
+            while (w >= base + all) {
+                if (chunk + 32 >= a.num_seqs) { more = false; break; }
+                base += all; chunk += 32;
+                load_chunk();
+            }
+            uint32_t vals[13] = {0};
+            if (more) {
+                const uint32_t k = __ffs(__ballot_sync(0xffffffffu, w < base + upto)) - 1;
+                const uint32_t seq = chunk + k, rem = w - base - __shfl_sync(0xffffffffu, upto - mine, k);
+                const uint32_t q0 = __shfl_sync(0xffffffffu, qs, k), len = __shfl_sync(0xffffffffu, T_s, k);
+                const uint32_t blk = (len + TPI - 1) / TPI - 1 - rem / a.nkv;
+                const uint32_t tok0 = q0 + blk * TPI, ntok = min(TPI, len - blk * TPI);
+                const uint32_t L = min(__ldg(a.kv_lens + seq), 0x7fffff00u);
+                const int32_t pos0 = (int32_t)L - (int32_t)len + (int32_t)(blk * TPI), p_hi = pos0 + (int32_t)ntok - 1;
+                uint32_t lo = 0;   // first row that a token of the item may see
+                if (a.rule.doc) {
+                    lo = 0xffffffffu;
+                    for (uint32_t t = lane; t < ntok; t += 32) {
+                        const uint32_t d = __ldg(a.rule.doc + tok0 + t);
+                        if (pos0 + (int32_t)t >= 0) lo = min(lo, d);
+                    }
+                    lo = __reduce_min_sync(0xffffffffu, lo);
+                }
+                const uint32_t pre = a.rule.prefix ? min(__ldg(a.rule.prefix + seq), L) : 0u;
+                const uint32_t p_lo = (uint32_t)max(pos0, 0);
+                uint32_t a0 = 0, na = 0, b0 = 0, n = 0;
+                if (p_hi >= 0 && lo < L) {
+                    const uint32_t wlo = max(lo, a.rule.window && p_lo + 1 > a.rule.window ? p_lo + 1 - a.rule.window : 0u);
+                    const uint32_t tb0 = wlo / N, tb1 = wlo <= (uint32_t)p_hi ? (uint32_t)p_hi / N + 1 : tb0;
+                    const uint32_t ta0 = lo / N, ta1 = lo < pre ? (pre - 1) / N + 1 : ta0;
+                    if (ta1 == ta0) { b0 = tb0; n = tb1 - tb0; }
+                    else if (tb1 == tb0 || ta1 >= tb0) { b0 = ta0; n = max(ta1, tb1) - ta0; }
+                    else { a0 = ta0; na = ta1 - ta0; b0 = tb0; n = na + tb1 - tb0; }
+                }
+                const uint32_t row0 = a.kv_starts ? __ldg(a.kv_starts + seq) : (uint32_t)min(seq * a.seq_rows, 0x7fffff00ull);
+                const uint32_t v[13] = {1u, seq, rem % a.nkv, tok0, ntok, (uint32_t)pos0, L, row0, a0, na, b0, n, pre};
+#pragma unroll
+                for (int i = 0; i < 13; ++i) vals[i] = v[i];
+            }
+            if (ic >= 2) ok = mbar_wait(bar(B_IEMPTY + (ic & 1)), ((ic >> 1) - 1) & 1, wc, 31);
+            if (!ok) break;
+            if (lane == 0) {
+#pragma unroll
+                for (int i = 0; i < 13; ++i) items[16 * (ic & 1) + i] = vals[i];
+                mbar_arrive(bar(B_IFULL + (ic & 1)));
+            }
+            __syncwarp();
+        }
+    } else if (warp == kWProd) {
+        // =============================== TMA producer ===============================
+        if (lane == 0) {
+            bool ok = true;
+            uint32_t gk = 0, gv = 0, qn[2] = {0, 0};   // K and V tiles, Q tiles of each row tile requested so far
+            Item it{};
+            auto load_kv = [&](uint32_t dst, const CUtensorMap *map, uint32_t b, uint32_t k0) {
+                if (a.page_table) {
+                    for (uint32_t r = 0; r < N; r += a.box_rows) {   // a box never leaves its page; past the sequence: a page that does not exist reads as zero
+                        const uint32_t row = k0 + r, pi = row / a.page_rows;
+                        const int page = row < it.L && pi < a.max_pages ? (int)__ldg(a.page_table + (size_t)it.seq * a.max_pages + pi) : -1;
+#pragma unroll
+                        for (uint32_t c = 0; c < C::kSlabs; ++c)
+                            tma_load_4d(dst + c * C::kKvSlab + r * 128u, map, b, 64 * c, (int)it.kvh, (int)(row % a.page_rows), page);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t c = 0; c < C::kSlabs; ++c) tma_load_4d(dst + c * C::kKvSlab, map, b, 64 * c, (int)it.kvh, (int)(it.row0 + k0), 0);
+                }
+            };
+            auto load_k = [&](uint32_t j) {
+                const uint32_t s = gk % C::kKS;
+                if (gk >= C::kKS && !mbar_wait(bar(B_KEMPTY + s), (gk / C::kKS - 1) & 1, wc, 32)) return false;
+                mbar_expect_tx(bar(B_KFULL + s), C::kKvTile);
+                load_kv(smem_base + C::kSmemK + s * C::kKvTile, &map_k, bar(B_KFULL + s), it.tile(j) * N);
+                ++gk;
+                return true;
+            };
+            auto load_v = [&](uint32_t j) {
+                const uint32_t s = gv % C::kVS;
+                if (gv >= C::kVS && !mbar_wait(bar(B_VEMPTY + s), (gv / C::kVS - 1) & 1, wc, 33)) return false;
+                mbar_expect_tx(bar(B_VFULL + s), C::kKvTile);
+                load_kv(smem_base + C::kSmemV + s * C::kKvTile, &map_v, bar(B_VFULL + s), it.tile(j) * N);
+                ++gv;
+                return true;
+            };
+            for (uint32_t ic = 0; ok && take_item(ic, it, kThreadRole, 34); ++ic) {
+                if (!it.n) continue;
+                for (uint32_t q = 0; q < NT && ok; ++q) {
+                    if (q * TPT >= it.ntok) continue;
+                    if (qn[q] > 0) ok = mbar_wait(bar(B_QEMPTY + q), (qn[q] - 1) & 1, wc, 35);
+                    if (!ok) break;
+                    ++qn[q];
+                    mbar_expect_tx(bar(B_QFULL + q), C::kSlabs * R * 128u);
+#pragma unroll
+                    for (uint32_t c = 0; c < C::kSlabs; ++c)
+                        tma_load_3d(smem_base + q * C::kQTile + c * C::kQSlab, &map_q, bar(B_QFULL + q), 64 * c, (int)(it.kvh * a.G), (int)(it.tok0 + q * TPT));
+                }
+                // K runs kAhead + 1 tiles in front of V, as the score MMAs run in front of the PV MMAs
+                for (uint32_t j = 0; j < it.n + C::kAhead && ok; ++j) {
+                    if (j < it.n) ok = load_k(j);
+                    if (ok && j + 1 > C::kAhead) ok = load_v(j - C::kAhead);
+                }
+            }
+            if (*abort_word || gave_up(a.status)) {   // copies may be in flight: a bounded time for them to land before the memory is handed back
+                for (uint32_t s = 0; s < C::kKS; ++s)
+                    for (uint32_t i = 0; gk > s && i < (1u << 16) && !mbar_try(bar(B_KFULL + s), ((gk - 1 - s) / C::kKS) & 1); ++i) {}
+                for (uint32_t s = 0; s < C::kVS; ++s)
+                    for (uint32_t i = 0; gv > s && i < (1u << 16) && !mbar_try(bar(B_VFULL + s), ((gv - 1 - s) / C::kVS) & 1); ++i) {}
+                for (uint32_t q = 0; q < NT; ++q)
+                    for (uint32_t i = 0; qn[q] && i < (1u << 16) && !mbar_try(bar(B_QFULL + q), (qn[q] - 1) & 1); ++i) {}
+            }
+        }
+    } else if (warp == kWFix) {
+        // =============================== rows past the sequence's end in its last V tile ===============================
+        // The issuer asks for it once the tile has landed (this warp does not follow the V ring, whose barriers' parity
+        // only tells neighbouring uses of a slot apart).
+        bool ok = true;
+        uint32_t gv = 0, fixes = 0;
+        Item it{};
+        for (uint32_t ic = 0; ok && take_item(ic, it, kWarpRole, 36); ++ic) {
+            if (!it.n) continue;
+            const uint32_t k0 = it.tile(it.n - 1) * N, s = (gv + it.n - 1) % C::kVS;
+            gv += it.n;
+            if (k0 + N <= it.L) continue;
+            ok = mbar_wait(bar(B_VREQ), fixes++ & 1, wc, 37);
+            if (!ok) break;
+            const uint32_t r0 = it.L - k0;   // (the last tile holds a row below L)
+#pragma unroll
+            for (uint32_t c = 0; c < C::kSlabs; ++c) {
+                uint4 *p = reinterpret_cast<uint4 *>(smem + C::kSmemV + s * C::kKvTile + c * C::kKvSlab + r0 * 128);
+                for (uint32_t i = lane; i < (N - r0) * 8; i += 32) p[i] = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_VFIX));
+        }
+    } else {
+        // =============================== MMA issuer ===============================
+        if (lane == 0) {
+            const uint32_t idesc_qk = make_idesc(kFmt, false, N), idesc_pv = make_idesc(kFmt, true, HD);
+            bool ok = true;
+            uint32_t gk = 0, gv = 0, qn[2] = {0, 0}, sc[2] = {0, 0}, pc[2] = {0, 0}, fixes = 0;
+            Item it{};
+            bool fix = false;
+            auto issue_s = [&](uint32_t q, uint32_t b, uint32_t s) {   // scores of row tile q into buffer b from K slot s
+                const uint32_t qa = smem_base + q * C::kQTile, kb = smem_base + C::kSmemK + s * C::kKvTile;
+#pragma unroll
+                for (uint32_t ks = 0; ks < HD / 16; ++ks) {
+                    const uint32_t so = ks >> 2, ko = (ks & 3) * 32;
+                    mma_ss(tmem + b * N, desc_kmajor(qa + so * C::kQSlab + ko), desc_kmajor(kb + so * C::kKvSlab + ko), idesc_qk, ks > 0);
+                }
+                tc_commit(bar(B_SFULL + b));
+            };
+            auto issue_pv = [&](uint32_t q, uint32_t b, uint32_t s, bool first) {
+                const uint32_t vb = smem_base + C::kSmemV + s * C::kKvTile;
+#pragma unroll
+                for (uint32_t ks = 0; ks < N / 16; ++ks)
+                    mma_ts(tmem + C::kColO + q * 128, tmem + b * N + ks * 8, desc_mnmajor(vb + ks * 2048, C::kKvSlab), idesc_pv, !first || ks > 0);
+            };
+            auto wait_k = [&]() { return mbar_wait(bar(B_KFULL + gk % C::kKS), (gk / C::kKS) & 1, wc, 38); };
+            auto wait_v = [&](uint32_t j) {   // tile j of the item has landed, and been cleared past the sequence's end
+                if (!mbar_wait(bar(B_VFULL + gv % C::kVS), (gv / C::kVS) & 1, wc, 39)) return false;
+                if (!fix || j + 1 != it.n) return true;
+                mbar_arrive(bar(B_VREQ));
+                ++fixes;
+                return mbar_wait(bar(B_VFIX), (fixes - 1) & 1, wc, 40);
+            };
+            for (uint32_t ic = 0; ok && take_item(ic, it, kThreadRole, 41); ++ic) {
+                const uint32_t n = it.n;
+                if (!n) continue;
+                fix = (it.tile(n - 1) + 1) * N > it.L;
+                ok = mbar_wait(bar(B_QFULL), qn[0]++ & 1, wc, 42);
+                if (!ok) break;
+                if constexpr (NT == 2) {
+                    // order per K/V tile: S0(j), PV1(j-1), S1(j), PV0(j); the pipe works on one row tile while the other is in its
+                    // softmax.  A commit covers all MMAs issued before it, so S_q(j) complete says PV_q(j-1) complete.
+                    const bool two = it.ntok > TPT;
+                    for (uint32_t j = 0; j <= n && ok; ++j) {
+                        if (j < n) {
+                            if (!(ok = wait_k())) break;
+                            tc_fence_after();
+                            issue_s(0, 0, gk % C::kKS);
+                            if (j == n - 1) tc_commit(bar(B_QEMPTY));
+                            if (!two) { tc_commit(bar(B_KEMPTY + gk % C::kKS)); ++gk; }
+                        }
+                        if (two && j >= 1) {   // V of tile j-1 has been waited for
+                            if (!(ok = mbar_wait(bar(B_PFULL + 1), pc[1]++ & 1, wc, 43))) break;
+                            tc_fence_after();
+                            issue_pv(1, 1, gv % C::kVS, j == 1);
+                            tc_commit(bar(B_VEMPTY + gv % C::kVS));
+                            ++gv;
+                            if (j == n) tc_commit(bar(B_OFULL + 1));
+                        }
+                        if (j < n) {
+                            if (two) {
+                                if (j == 0) {
+                                    if (!(ok = mbar_wait(bar(B_QFULL + 1), qn[1]++ & 1, wc, 44))) break;
+                                    tc_fence_after();
+                                }
+                                issue_s(1, 1, gk % C::kKS);
+                                tc_commit(bar(B_KEMPTY + gk % C::kKS));
+                                ++gk;
+                                if (j == n - 1) tc_commit(bar(B_QEMPTY + 1));
+                            }
+                            if (!(ok = wait_v(j))) break;
+                            if (!(ok = mbar_wait(bar(B_PFULL), pc[0]++ & 1, wc, 45))) break;
+                            tc_fence_after();
+                            issue_pv(0, 0, gv % C::kVS, j == 0);
+                            if (!two) { tc_commit(bar(B_VEMPTY + gv % C::kVS)); ++gv; }
+                            if (j == n - 1) tc_commit(bar(B_OFULL));
+                        }
+                    }
+                } else {
+                    // one row tile, kAhead score tiles in front of the PV; the buffer of S(j + kAhead) held P(j - 1), whose PV was
+                    // issued before (MMAs of one thread execute in order)
+                    auto score = [&](uint32_t j) {
+                        if (!wait_k()) return false;
+                        tc_fence_after();
+                        issue_s(0, sc[0] % NS, gk % C::kKS);
+                        tc_commit(bar(B_KEMPTY + gk % C::kKS));
+                        ++gk; ++sc[0];
+                        if (j == n - 1) tc_commit(bar(B_QEMPTY));
+                        return true;
+                    };
+                    for (uint32_t j = 0; j < min(C::kAhead, n) && ok; ++j) ok = score(j);
+                    for (uint32_t j = 0; j < n && ok; ++j) {
+                        if (j + C::kAhead < n && !(ok = score(j + C::kAhead))) break;
+                        if (!(ok = wait_v(j))) break;
+                        if (!(ok = mbar_wait(bar(B_PFULL + pc[0] % NS), (pc[0] / NS) & 1, wc, 45))) break;
+                        tc_fence_after();
+                        issue_pv(0, pc[0] % NS, gv % C::kVS, j == 0);
+                        tc_commit(bar(B_VEMPTY + gv % C::kVS));
+                        tc_commit(bar(B_PVDONE + pc[0] % NS));
+                        ++pc[0];
+                        ++gv;
+                        if (j == n - 1) tc_commit(bar(B_OFULL));
+                    }
+                }
+            }
+        }
+    }
+    } else {
+        if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        // =============================== softmax (one thread per row) ===============================
+        const uint32_t q = warp >> 2, r = tid & 127;
+        const uint32_t t_lane = tmem + (((warp & 3) * 32) << 16);
+        const uint32_t t_o = t_lane + C::kColO + q * 128;
+        const uint32_t t_rel = q * TPT + r / a.G, g = r % a.G;
+        const float scale2 = a.rule.scale * kRuleLog2e;
+        const float cap_in = a.rule.scale * a.rule.inv_cap * (2.0f * kRuleLog2e), cap2 = a.rule.cap * kRuleLog2e;
+        bool ok = true;
+        uint32_t cnt = 0, oc = 0;   // score tiles and items of this row tile so far (barrier phases)
+        Item it{};
+        for (uint32_t ic = 0; ok && take_item(ic, it, kWarpRole, 46); ++ic) {
+            if (q * TPT >= it.ntok) continue;
+            const bool live = r < R && t_rel < it.ntok;
+            const int32_t pos = it.pos0 + (int32_t)t_rel;
+            const uint32_t head = it.kvh * a.G + g;
+            int32_t c_lo = 0, c_hi = 0, p_lo = 0, p_hi = 0;   // rows [c_lo, c_hi) and [p_lo, p_hi) are seen
+            if (live && pos >= 0) {
+                p_lo = a.rule.doc ? (int32_t)min(__ldg(a.rule.doc + it.tok0 + t_rel), 0x7fffffffu) : 0;
+                p_hi = (int32_t)it.pre;
+                c_hi = pos + 1;
+                c_lo = max(p_lo, a.rule.window && (uint32_t)c_hi > a.rule.window ? c_hi - (int32_t)a.rule.window : 0);
+            }
+            float slope2 = 0.f;
+            if (MODE == 2) slope2 = live ? __ldg(a.rule.slopes + head) * kRuleLog2e : 0.f;
+            float m_ref = -INFINITY, l_sum = 0.f;
+            for (uint32_t j = 0; j < it.n && ok; ++j) {
+                const uint32_t b = NT == 2 ? q : cnt % NS;
+                ok = mbar_wait(bar(B_SFULL + b), (NT == 2 ? cnt : cnt / NS) & 1, wc, 47);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t t_s = t_lane + b * N;
+                const int32_t k0 = (int32_t)(it.tile(j) * N);
+                uint32_t x[N / 32][32];
+#pragma unroll
+                for (uint32_t c = 0; c < N / 32; ++c) tmem_ld32(t_s + c * 32, x[c]);
+                // (a row without a token may hold and become anything)
+                const bool whole = !live || (c_lo <= k0 && c_hi >= k0 + (int32_t)N) || (p_lo <= k0 && p_hi >= k0 + (int32_t)N);
+                tmem_wait_ld();
+                // ---- the rule: x = z log2(e), or with scale alone the raw product ----
+                if (MODE != 0) {
+#pragma unroll
+                    for (uint32_t c = 0; c < N / 32; ++c)
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; i += 2) {
+                            float y0 = __uint_as_float(x[c][i]), y1 = __uint_as_float(x[c][i + 1]);
+                            if (MODE == 1 || a.rule.cap > 0.f) {
+                                // 1 - 2/(1 + e), one reciprocal for two elements; at e = 2^60 the tanh is 1 to the last bit
+                                const float e0 = 1.0f + rule_exp2(fminf(y0 * cap_in, 60.f)), e1 = 1.0f + rule_exp2(fminf(y1 * cap_in, 60.f));
+                                const float rr = rule_rcp(e0 * e1) * (-2.0f * cap2);
+                                y0 = fmaf(rr, e1, cap2); y1 = fmaf(rr, e0, cap2);
+                            } else {
+                                y0 *= scale2; y1 *= scale2;
+                            }
+                            if (MODE == 2) {
+                                const float d = (float)(pos - k0 - (int32_t)(c * 32 + i));
+                                y0 = fmaf(-slope2, fabsf(d), y0); y1 = fmaf(-slope2, fabsf(d - 1.0f), y1);
+                            }
+                            x[c][i] = __float_as_uint(y0); x[c][i + 1] = __float_as_uint(y1);
+                        }
+                }
+                if (!__all_sync(0xffffffffu, whole)) {
+#pragma unroll
+                    for (uint32_t c = 0; c < N / 32; ++c) {
+                        const int32_t kc = k0 + (int32_t)(c * 32);
+                        const uint32_t see = bit_range(c_lo - kc, c_hi - kc) | bit_range(p_lo - kc, p_hi - kc);
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; ++i)
+                            if (!(see & (1u << i))) x[c][i] = 0xff800000u;   // -inf
+                    }
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (uint32_t c = 0; c < N / 32; ++c)
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i += 2)
+                        mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                if (MODE == 0) mx *= scale2;   // scale > 0
+                // ---- lazy rescale of O and l ----
+                float corr = 1.f;
+                if (j == 0) {
+                    m_ref = mx;
+                } else if (mx > m_ref + 8.0f) {
+                    corr = rule_exp2(m_ref - mx);
+                    m_ref = mx;
+                }
+                if (__any_sync(0xffffffffu, corr != 1.f)) {
+                    // the PV of the tile before must have written O (its buffer's own barrier: the PVs of up to kAhead tiles may be under way)
+                    if (NT == 1) ok = mbar_wait(bar(B_PVDONE + (cnt - 1) % NS), ((cnt - 1) / NS) & 1, wc, 48);
+                    if (!ok) break;
+                    if (NT == 1) tc_fence_after();
+                    l_sum *= corr;
+#pragma unroll 1
+                    for (uint32_t c = 0; c < HD / 16; ++c) {
+                        uint32_t v[16];
+                        tmem_ld16(t_o + c * 16, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+                        tmem_st16(t_o + c * 16, v);
+                    }
+                }
+                // ---- P = 2^(x - m), row sum, packed over S ----
+                const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;   // nothing seen yet: every weight is 2^-inf
+                const float mul = MODE == 0 ? scale2 : 1.0f;
+                const unsigned long long mul2 = pack_f32x2(mul, mul), negm2 = pack_f32x2(neg_m, neg_m);
+                unsigned long long ls2[2] = {0ull, 0ull};
+#pragma unroll
+                for (uint32_t c = 0; c < N / 32; ++c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i += 2) {
+                        float x0, x1;
+                        fma_f32x2(x0, x1, __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]), mul2, negm2);
+                        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                        ls2[(i >> 1) & 1] = add_f32x2(ls2[(i >> 1) & 1], pack_f32x2(p0, p1));
+                        pk[i >> 1] = pack16<T>(p0, p1);
+                    }
+                    tmem_st16(t_s + c * 16, pk);
+                }
+                float s0, s1, s2, s3;
+                asm("mov.b64 {%0, %1}, %2;" : "=f"(s0), "=f"(s1) : "l"(ls2[0]));
+                asm("mov.b64 {%0, %1}, %2;" : "=f"(s2), "=f"(s3) : "l"(ls2[1]));
+                l_sum += (s0 + s1) + (s2 + s3);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(bar(B_PFULL + b));
+                ++cnt;
+            }
+            // ---- epilogue: O / l, lse ----
+            if (it.n && ok) {
+                ok = mbar_wait(bar(B_OFULL + q), oc & 1, wc, 49);
+                ++oc;
+                if (ok) tc_fence_after();
+            }
+            if (!ok) break;
+            const bool seen = l_sum > 0.f;
+            const float inv = seen ? 1.0f / l_sum : 0.f;
+            const size_t row = ((size_t)it.tok0 + t_rel) * a.nh + head;
+            T *dst = reinterpret_cast<T *>(a.out) + row * HD;
+#pragma unroll 2
+            for (uint32_t c = 0; c < HD / 32; ++c) {
+                uint32_t v[32];
+                if (it.n) {
+                    tmem_ld32(t_o + c * 32, v);
+                    tmem_wait_ld();
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = seen ? __float_as_uint(__uint_as_float(v[i]) * inv) : 0u;
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint4 w4;
+                        w4.x = pack16<T>(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                        w4.y = pack16<T>(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+                        w4.z = pack16<T>(__uint_as_float(v[i + 4]), __uint_as_float(v[i + 5]));
+                        w4.w = pack16<T>(__uint_as_float(v[i + 6]), __uint_as_float(v[i + 7]));
+                        *reinterpret_cast<uint4 *>(dst + c * 32 + i) = w4;
+                    }
+                }
+            }
+            if (live && a.lse) a.lse[row] = seen ? (m_ref + log2f(l_sum)) * kRuleLn2 : -INFINITY;
+            tc_fence_before();   // the reads of O are ordered before the arrival that lets the next item's PV write it
+        }
+    }
+    // ---- teardown: everyone arrives, TMEM goes back ----
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kWMma) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// cuTensorMapEncodeTiled is looked up through the runtime, so that the library does not link against libcuda
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                             const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<EncodeFn>(p) : nullptr;
+    }();
+    return fn;
+}
+static bool encode(CUtensorMap *map, uint32_t dtype, const void *base, uint32_t rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    EncodeFn fn = encode_fn();
+    return fn && fn(map, dtype == SHADY_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(base), dims,
+                    strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Maps { CUtensorMap q, k, v; };
+
+template <typename T, int HD, int MODE> static int launch(shady_ctx *ctx, const Maps &m, const Args &a, uint32_t blocks) {
+    using C = Cfg<HD>;
+    auto kern = prefill_rule_kernel<T, HD, MODE>;
+    SHADY_CUDA_OK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    if (C::kNT == 2) {   // a build that launches with fewer registers would wait for them for good
+        cudaFuncAttributes at{};
+        SHADY_CUDA_OK(ctx, cudaFuncGetAttributes(&at, kern));
+        SHADY_REQUIRE(ctx, at.numRegs >= (int)kRegsLaunch, SHADY_ERR_UNSUPPORTED, "prefill_rule: this build launches with too few registers per thread");
+    }
+    kern<<<blocks, C::kThreads, C::kSmem, ctx->stream>>>(m.q, m.k, m.v, a);
+    ctx->launches++;
+    SHADY_CUDA_OK(ctx, cudaGetLastError());
+    return SHADY_OK;
+}
+template <typename T, int HD> static int launch_mode(shady_ctx *ctx, const Maps &m, const Args &a, uint32_t blocks) {
+    if (a.rule.slopes) return launch<T, HD, 2>(ctx, m, a, blocks);
+    if (a.rule.cap > 0.f) return launch<T, HD, 1>(ctx, m, a, blocks);
+    return launch<T, HD, 0>(ctx, m, a, blocks);
 }
 
 }  // namespace pr
@@ -95,24 +666,35 @@ int launch_prefill_rule(shady_ctx *ctx, const shady_prefill_params *p, const sha
         SHADY_REQUIRE(ctx, cache->seq_stride % row == 0, SHADY_ERR_BAD_ARG, w + ": seq_stride must be a whole number of cache rows");
     }
     if (!total_q) return SHADY_OK;
-    a.q = d_q; a.out = d_out; a.lse = d_lse; a.k_base = kv.k_base; a.v_base = kv.v_base;
+    if (const int st = pending_timeout(ctx, "prefill_rule")) return st;
+    a.status = status_ref(ctx); a.wait_mbar = ctx->wait_mbar;
+    a.out = d_out; a.lse = d_lse;
     a.page_table = kv.page_table; a.page_rows = kv.page_rows; a.max_pages = kv.max_pages;
-    a.seq_rows = cache->seq_stride / row; a.cache_rows = cache_rows;
+    a.seq_rows = cache->seq_stride / row;
     a.q_starts = d_q_starts; a.kv_starts = d_kv_starts; a.kv_lens = d_kv_lens;
     a.num_seqs = p->num_seqs; a.total_q = total_q; a.nkv = p->num_kv_heads; a.nh = p->num_q_heads; a.G = G;
-    const unsigned long long blocks = ((unsigned long long)total_q * a.nh + 3) / 4;
-    SHADY_REQUIRE(ctx, blocks <= 0x7fffffffull, SHADY_ERR_UNSUPPORTED, w + ": too many tokens");
-    auto go = [&](auto kern) { kern<<<(unsigned)blocks, 128, 0, ctx->stream>>>(a); };
-    if (p->dtype == SHADY_F16) {
-        if (p->head_dim == 128) go(pr::prefill_rule_kernel<__half, 128>);
-        else go(pr::prefill_rule_kernel<__half, 256>);
-    } else {
-        if (p->head_dim == 128) go(pr::prefill_rule_kernel<__nv_bfloat16, 128>);
-        else go(pr::prefill_rule_kernel<__nv_bfloat16, 256>);
+    const uint32_t hd = p->head_dim, tile = hd == 128 ? pr::Cfg<128>::kN : pr::Cfg<256>::kN, nt = hd == 128 ? pr::Cfg<128>::kNT : pr::Cfg<256>::kNT;
+    const uint32_t tpt = 128 / G;   // tokens of a row tile
+    pr::Maps m;
+    {
+        const cuuint64_t dims[3] = {hd, p->num_q_heads, total_q}, strides[2] = {hd * 2ull, (cuuint64_t)p->num_q_heads * hd * 2};
+        const cuuint32_t box[3] = {64, G, tpt};
+        bool fine = pr::encode(&m.q, p->dtype, d_q, 3, dims, strides, box);
+        uint32_t rows = tile;   // rows of a box: a tile, or the largest power of two that divides both a tile and a page
+        while (kv.page_table && kv.page_rows % rows) rows /= 2;
+        a.box_rows = rows;
+        const cuuint64_t pages = kv.page_table ? cache_rows / kv.page_rows : 1, per = kv.page_table ? kv.page_rows : cache_rows;
+        const cuuint64_t kd[4] = {hd, p->num_kv_heads, per, pages}, ks[3] = {hd * 2ull, row * 2, pages > 1 ? per * row * 2 : row * 2};
+        const cuuint32_t kb[4] = {64, 1, rows, 1};
+        fine = fine && pr::encode(&m.k, p->dtype, kv.k_base, 4, kd, ks, kb) && pr::encode(&m.v, p->dtype, kv.v_base, 4, kd, ks, kb);
+        SHADY_REQUIRE(ctx, fine, SHADY_ERR_CUDA, w + ": cuTensorMapEncodeTiled failed");
     }
-    ctx->launches++;
-    SHADY_CUDA_OK(ctx, cudaGetLastError());
-    return SHADY_OK;
+    // items: blocks of nt * tpt tokens; a sequence's last block may be partly filled
+    const unsigned long long most = ((unsigned long long)total_q / (nt * tpt) + p->num_seqs) * p->num_kv_heads;
+    SHADY_REQUIRE(ctx, most <= 0x3fffffffull, SHADY_ERR_UNSUPPORTED, w + ": too many tokens");
+    const uint32_t blocks = (uint32_t)(most < (unsigned long long)ctx->num_sms ? most : (unsigned long long)ctx->num_sms);
+    if (p->dtype == SHADY_F16) return hd == 128 ? pr::launch_mode<__half, 128>(ctx, m, a, blocks) : pr::launch_mode<__half, 256>(ctx, m, a, blocks);
+    return hd == 128 ? pr::launch_mode<__nv_bfloat16, 128>(ctx, m, a, blocks) : pr::launch_mode<__nv_bfloat16, 256>(ctx, m, a, blocks);
 }
 
 }  // namespace shady
