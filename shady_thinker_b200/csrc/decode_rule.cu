@@ -50,6 +50,7 @@ namespace dr {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32, kBlock = 16, kHeads = 8;
 constexpr uint32_t kMinShare = kWarps;   // blocks: one per warp
+constexpr int kMaxSms = 160;             // a unit has at most one record per resident CTA
 
 struct Args {
     RuleArgs rule;
@@ -60,7 +61,7 @@ struct Args {
     float *lse;
     const uint32_t *lens;
     uint32_t *counters;   // [num_seqs][nkv * groups]
-    float *records;       // [2 * grid][kHeads][HD + 2]
+    float *records;       // [2 * grid]: see kRec
     uint32_t num_seqs, nkv, G, nh, groups, q_dtype, out_dtype;
 };
 
@@ -124,6 +125,7 @@ template <int HD, bool Q8> struct Smem {
     static constexpr int kMisc = 2 * kWarps * kHeads * 4 + kHeads * 4 + 16;
     static constexpr int kTotal = kQ + kRing + kMisc;
     static_assert(kWarps * kMergeTile <= kRing, "the merge tiles reuse the rings");
+    static_assert(kMaxSms * kCtas * kHeads * 4 <= kRing, "so do the factors of all records of a unit");
 };
 
 // What one sequence puts on the line.
@@ -147,6 +149,19 @@ __device__ __forceinline__ Seq seq_of(const Args &a, uint32_t s) {
     return q;
 }
 __device__ __forceinline__ bool visible(const Seq &q, uint32_t row) { return row < q.L && row >= q.doc && (row >= q.wlo || row < q.pre); }
+
+// four output elements of a head from the weighted sum o and the sum of the weights l
+template <int HD> __device__ __forceinline__ void put_out(const Args &a, uint32_t seq, uint32_t head, uint32_t d, const float4 &o, float l) {
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const float v[4] = {l > 0.f ? o.x * inv : 0.f, l > 0.f ? o.y * inv : 0.f, l > 0.f ? o.z * inv : 0.f, l > 0.f ? o.w * inv : 0.f};
+    const size_t at = ((size_t)seq * a.nh + head) * HD + d;
+    if (a.out_dtype == SHADY_F32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+    else if (a.out_dtype == SHADY_F16) *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(a.out) + at) = make_uint2(pack<__half>(v[0], v[1]), pack<__half>(v[2], v[3]));
+    else *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + at) = make_uint2(pack<__nv_bfloat16>(v[0], v[1]), pack<__nv_bfloat16>(v[2], v[3]));
+}
+__device__ __forceinline__ void put_lse(const Args &a, uint32_t seq, uint32_t head, float m, float l) {
+    if (a.lse) a.lse[(size_t)seq * a.nh + head] = l > 0.f ? (m + log2f(l)) * kRuleLn2 : -INFINITY;
+}
 
 template <typename T, int HD, bool Q8>
 __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_kernel(const __grid_constant__ Args a) {
@@ -214,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
             }
         }
         auto row_of_block = [&](uint32_t b) { return (b < sq.na ? sq.a0 + b : sq.b0 + (b - sq.na)) * kBlock; };
-        const uint32_t l_row = lane / CH % RPI, l_chunk = lane % CH;
+        const uint32_t l_row = lane / CH % RPI, l_chunk = lane % CH, l_sw = l_chunk ^ S::swz(l_row);
         // row numbers of the caches are taken relative to a base that the block's page or sequence gives
         auto issue = [&](uint32_t i) {
             const uint32_t r0 = row_of_block(p0 + warp + i * kWarps);
@@ -233,19 +248,20 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                     row0 = r0;
                 }
             }
-            const size_t stride = (size_t)a.nkv * S::kRow;
+            // a block inside the window or the prefix needs no test per row
+            const bool full = have && ((r0 >= sq.wlo && r0 + kBlock <= sq.L) || (r0 >= sq.doc && r0 + kBlock <= sq.pre));
+            const size_t stride = (size_t)a.nkv * S::kRow, off = (size_t)(row0 + l_row) * stride + (size_t)kvh * S::kRow + l_chunk * 16;
 #pragma unroll
             for (int k = 0; k < NI; ++k) {
-                const uint32_t r = k * RPI + l_row;
-                const bool ok = have && visible(sq, r0 + r);
-                const size_t off = ok ? (size_t)(row0 + r) * stride + (size_t)kvh * S::kRow + l_chunk * 16 : 0;
-                const uint32_t so = r * S::kRow + ((l_chunk ^ S::swz(r)) << 4);
-                cp16(st + so, kb + off, ok);
-                cp16(st + S::kTile + so, vb + off, ok);
+                const bool ok = full || (have && visible(sq, r0 + k * RPI + l_row));
+                const uint32_t so = (k * RPI + l_row) * S::kRow + ((l_sw ^ S::swz(k * RPI)) << 4);   // swz(a + b) = swz(a) ^ swz(b) here: no common bits
+                const size_t o = ok ? off + (size_t)(k * RPI) * stride : 0;
+                cp16(st + so, kb + o, ok);
+                cp16(st + S::kTile + so, vb + o, ok);
             }
             if constexpr (Q8) {
                 const uint32_t r = lane & 15;
-                const bool ok = have && visible(sq, r0 + r);
+                const bool ok = full || (have && visible(sq, r0 + r));
                 const float *sc = lane < 16 ? a.rq.k_scales : a.rq.v_scales;
                 cp4(st + 2 * S::kTile + lane * 4, sc + (ok ? (size_t)(row0 + r) * a.nkv + kvh : 0), ok);
             }
@@ -321,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
             const uint32_t st = ring + (i % ST) * S::kStage;
             const uint32_t r0 = row_of_block(p0 + warp + i * kWarps);
             // ---- S^T: 16 positions x 8 heads ----
-            float sT[4] = {0.f, 0.f, 0.f, 0.f};
+            float s2[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // two chains of products: half the dependent MMAs
             if constexpr (Q8) {
 #pragma unroll
                 for (int c = 0; c < CH; c += 2) {
@@ -332,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t ka[4] = {codes_to_f16<0x10>(kb[2 * h]), codes_to_f16<0x10>(kb[2 * h + 1]),
                                                 codes_to_f16<0x32>(kb[2 * h]), codes_to_f16<0x32>(kb[2 * h + 1])};
-                        mma<T>(sT, ka, qb[c + h][0], qb[c + h][1]);
+                        mma<T>(s2[h], ka, qb[c + h][0], qb[c + h][1]);
                     }
                 }
             } else {
@@ -341,9 +357,10 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                     uint32_t ka[4];   // (pos 0-7, chunk 2c), (pos 8-15, chunk 2c), (pos 0-7, chunk 2c+1), (pos 8-15, chunk 2c+1)
                     const uint32_t ch = 2 * c + (mat >> 1), r = (mat & 1) * 8 + rin;
                     ldm4(ka, st + r * S::kRow + ((ch ^ S::swz(r)) << 4));
-                    mma<T>(sT, ka, qb[c][0], qb[c][1]);
+                    mma<T>(s2[c & 1], ka, qb[c][0], qb[c][1]);
                 }
             }
+            const float sT[4] = {s2[0][0] + s2[1][0], s2[0][1] + s2[1][1], s2[0][2] + s2[1][2], s2[0][3] + s2[1][3]};
             // ---- the rule; this lane has positions g and g + 8 of heads 2t, 2t+1.  y = z log2(e) (+ log2 vs) ----
             float y[4], inv_vs[2] = {1.f, 1.f};
 #pragma unroll
@@ -435,30 +452,40 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
             tile[(2 * t) * S::kORow + dhi] = oT[c][2]; tile[(2 * t + 1) * S::kORow + dhi] = oT[c][3];
         }
         __syncthreads();
-        constexpr int kRec = HD + 2;
+        // record: O of the eight heads [kHeads][HD], then (maximum, sum) of each
+        constexpr int kRec = kHeads * (HD + 2);
         const uint32_t slot = 2 * blockIdx.x + (x == x_first ? 0u : 1u);
-        float *rec = a.records + (size_t)slot * kHeads * kRec;
-        for (uint32_t e = tid; e < heads * HD; e += kThreads) {
-            const uint32_t h = e / HD, d = e % HD;
-            float M = -INFINITY;
+        float *rec = a.records + (size_t)slot * kRec;
+        if (tid < kHeads) {   // the warps' factors, in place of their maxima, and the joint statistics
+            float m = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w * kHeads + h]);
-            const float mu = M == -INFINITY ? 0.f : M;
-            float o = 0.f, l = 0.f;
+            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm_m[w * kHeads + tid]);
+            const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float f = rule_exp2(sm_m[w * kHeads + h] - mu);
-                o += f * reinterpret_cast<const float *>(sm_ring + w * S::kMergeTile)[h * S::kORow + d];
-                l += f * sm_l[w * kHeads + h];
+                const float f = rule_exp2(sm_m[w * kHeads + tid] - mu);
+                sm_m[w * kHeads + tid] = f;
+                l += f * sm_l[w * kHeads + tid];
             }
+            sm_l[tid] = l;
             if (whole) {
-                const size_t row = (size_t)seq * a.nh + h0 + h;
-                store_from_f32(a.out, row * HD + d, a.out_dtype, l > 0.f ? o / l : 0.f);
-                if (d == 0 && a.lse) a.lse[row] = l > 0.f ? (M + log2f(l)) * kRuleLn2 : -INFINITY;
+                if (tid < heads) put_lse(a, seq, h0 + tid, m, l);
             } else {
-                rec[h * kRec + 2 + d] = o;
-                if (d == 0) { rec[h * kRec] = M; rec[h * kRec + 1] = l; }
+                *reinterpret_cast<float2 *>(rec + kHeads * HD + 2 * tid) = make_float2(m, l);
             }
+        }
+        __syncthreads();
+        for (uint32_t e = tid; e < heads * (HD / 4); e += kThreads) {
+            const uint32_t h = e / (HD / 4), d = e % (HD / 4) * 4;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = sm_m[w * kHeads + h];
+                const float4 v = *reinterpret_cast<const float4 *>(sm_ring + w * S::kMergeTile + (h * S::kORow + d) * 4);
+                o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+            }
+            if (whole) put_out<HD>(a, seq, h0 + h, d, o, sm_l[h]);
+            else *reinterpret_cast<float4 *>(rec + h * HD + d) = o;
         }
         if (!whole) {
             // ---- the last CTA to arrive joins the records of this (sequence, kv head, group) ----
@@ -472,35 +499,44 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                 if (tid == 0) a.counters[(size_t)seq * U + unit] = 0;
                 // share c0 wrote the piece as its last one (slot 1) unless the piece began with the share
                 const uint32_t slot0 = 2 * c0 + (u0 == c0 * share ? 0u : 1u);
-                auto record = [&](uint32_t k) { return a.records + (size_t)(k ? 2 * (c0 + k) : slot0) * kHeads * kRec; };
-                for (uint32_t e = tid; e < heads * HD; e += kThreads) {
-                    const uint32_t h = e / HD, d = e % HD;
-                    float M = -INFINITY, o = 0.f, l = 0.f;
-                    for (uint32_t k0 = 0; k0 < nrec; k0 += 8) {
-                        float rm[8], rl[8], ro[8];
-#pragma unroll
-                        for (uint32_t k = 0; k < 8; ++k) {
-                            rm[k] = -INFINITY; rl[k] = 0.f; ro[k] = 0.f;
-                            if (k0 + k < nrec) {
-                                const float *r = record(k0 + k) + h * kRec;
-                                rm[k] = __ldcg(r); rl[k] = __ldcg(r + 1); ro[k] = __ldcg(r + 2 + d);
-                            }
-                        }
-                        float mx = M;
-#pragma unroll
-                        for (uint32_t k = 0; k < 8; ++k) mx = fmaxf(mx, rm[k]);
-                        const float mu = mx == -INFINITY ? 0.f : mx, f0 = rule_exp2(M - mu);
-                        o *= f0; l *= f0;
-#pragma unroll
-                        for (uint32_t k = 0; k < 8; ++k) {
-                            const float f = rule_exp2(rm[k] - mu);
-                            o += f * ro[k]; l += f * rl[k];
-                        }
-                        M = mx;
+                auto record = [&](uint32_t k) { return a.records + (size_t)(k ? 2 * (c0 + k) : slot0) * kRec; };
+                float *sm_w = reinterpret_cast<float *>(sm_ring);   // the records' factors [nrec][kHeads]
+                // a warp finds the statistics of two heads: its lanes take the records
+                for (uint32_t h = warp; h < heads; h += kWarps) {
+                    float m = -INFINITY, l = 0.f;
+                    for (uint32_t k = lane; k < nrec; k += 32) {
+                        const float v = __ldcg(record(k) + kHeads * HD + 2 * h);
+                        sm_w[k * kHeads + h] = v;
+                        m = fmaxf(m, v);
                     }
-                    const size_t row = (size_t)seq * a.nh + h0 + h;
-                    store_from_f32(a.out, row * HD + d, a.out_dtype, l > 0.f ? o / l : 0.f);
-                    if (d == 0 && a.lse) a.lse[row] = l > 0.f ? (M + log2f(l)) * kRuleLn2 : -INFINITY;
+                    m = warp_max(m);
+                    const float mu = m == -INFINITY ? 0.f : m;
+                    for (uint32_t k = lane; k < nrec; k += 32) {
+                        const float f = rule_exp2(sm_w[k * kHeads + h] - mu);
+                        sm_w[k * kHeads + h] = f;
+                        l += f * __ldcg(record(k) + kHeads * HD + 2 * h + 1);
+                    }
+                    l = warp_sum(l);
+                    if (lane == 0) { sm_l[h] = l; put_lse(a, seq, h0 + h, m, l); }
+                }
+                __syncthreads();
+                for (uint32_t e = tid; e < heads * (HD / 4); e += kThreads) {
+                    const uint32_t h = e / (HD / 4), d = e % (HD / 4) * 4;
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                    constexpr uint32_t kUn = 16;   // records requested together
+                    for (uint32_t k0 = 0; k0 < nrec; k0 += kUn) {
+                        float4 v[kUn];
+#pragma unroll
+                        for (uint32_t k = 0; k < kUn; ++k)
+                            if (k0 + k < nrec) v[k] = __ldcg(reinterpret_cast<const float4 *>(record(k0 + k) + h * HD + d));
+#pragma unroll
+                        for (uint32_t k = 0; k < kUn; ++k)
+                            if (k0 + k < nrec) {
+                                const float f = sm_w[(k0 + k) * kHeads + h];
+                                o.x += f * v[k].x; o.y += f * v[k].y; o.z += f * v[k].z; o.w += f * v[k].w;
+                            }
+                    }
+                    put_out<HD>(a, seq, h0 + h, d, o, sm_l[h]);
                 }
             }
         }
@@ -514,6 +550,7 @@ static uint32_t head_groups(const shady_decode_params *p) { return (p->num_q_hea
 static int check(shady_ctx *ctx, const shady_decode_params *p) {
     SHADY_REQUIRE(ctx, p, SHADY_ERR_BAD_ARG, "decode_rule: null parameters");
     SHADY_REQUIRE(ctx, p->num_kv_heads && p->num_q_heads && p->num_seqs, SHADY_ERR_BAD_ARG, "decode_rule: zero-sized problem");
+    SHADY_REQUIRE(ctx, ctx->num_sms <= kMaxSms, SHADY_ERR_UNSUPPORTED, "decode_rule: more SMs than the merge is laid out for");
     SHADY_REQUIRE(ctx, p->num_q_heads % p->num_kv_heads == 0 && (!p->heads_per_kv || p->heads_per_kv == p->num_q_heads / p->num_kv_heads),
                   SHADY_ERR_BAD_ARG, "decode_rule: num_q_heads must be num_kv_heads * heads_per_kv");
     SHADY_REQUIRE(ctx, p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256, SHADY_ERR_UNSUPPORTED,
