@@ -15,9 +15,11 @@
 //   * A warp streams its own blocks with 16-byte cp.async into a ring of its own (rows that are not visible are
 //     filled with zeros and not read), the positions on the M rows of the MMA and eight heads on its N columns:
 //     S^T = K Q^T, O^T = V^T P^T, softmax statistics in f32 by shuffles.  Each cache byte is read once per eight heads.
-//   * Codes become f16 without a conversion instruction: a byte permute puts the byte c + 128 under 0x64, which is the
-//     f16 1024 + c + 128, and one subtraction of 1152 leaves c exactly.  ks multiplies the score; vs goes into the
-//     weight, whose running maximum is taken over z + ln(vs), so that the f16 weights stay within [0, 1] whatever
+//   * Codes become f16 without a conversion instruction.  V: a byte permute puts the byte c + 128 under 0x64, which is the
+//     f16 1024 + c + 128, and one subtraction of 1152 leaves c exactly.  K: the byte stays as it is, as the f16
+//     subnormal (c + 128) 2^-24, and 128 * sum(q) is taken off the product once per score (a dot product of head_dim
+//     terms bears the offset; a sum over a long context, V's, would not: its rounding errors all have one sign).
+//     ks multiplies the score; vs goes into the weight, whose running maximum is taken over z + ln(vs), so that the f16 weights stay within [0, 1] whatever
 //     the sizes of the scales; the sum of e^z divides by vs again in f32.
 //   * A share that holds only part of a (sequence, kv head, group) writes a record; the CTA that arrives last at its
 //     counter joins the records in the order of the shares, so the result does not depend on which CTA it was.
@@ -49,8 +51,13 @@ int fill_rule(shady_ctx *ctx, const shady_score_rule *rule, uint32_t head_dim, c
 namespace dr {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32, kBlock = 16, kHeads = 8;
+// Units without rows that follow the blocks of every (sequence, kv head, group) on the line: what ending one piece and
+// starting the next costs a CTA, so that shares are equal in time.  Ragged batch of 32 sequences, row-scaled: 0 units
+// 59 us, 8 53, 12 52, 16 51, 24 52; one sequence of 128k rows, head_dim 256: 67, 63, 60, 60, 60.
+constexpr uint32_t kPad = 16;
 constexpr uint32_t kMinShare = kWarps;   // blocks: one per warp
 constexpr int kMaxSms = 160;             // a unit has at most one record per resident CTA
+constexpr uint32_t kFlat = 12, kFan = 8; // records that one CTA joins at once, and size of a group where there are more
 
 struct Args {
     RuleArgs rule;
@@ -61,8 +68,10 @@ struct Args {
     float *lse;
     const uint32_t *lens;
     uint32_t *counters;   // [num_seqs][nkv * groups]
+    uint32_t *group_counters;   // [2 * grid], by the slot of a group's first record
     float *records;       // [2 * grid]: see kRec
     uint32_t num_seqs, nkv, G, nh, groups, q_dtype, out_dtype;
+    uint32_t pad;         // units without rows behind every unit's blocks
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool ok) {   // !ok: 16 bytes of zeros, nothing read
@@ -108,6 +117,11 @@ template <uint32_t SEL> __device__ __forceinline__ uint32_t codes_to_f16(uint32_
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
+// the same two bytes as they are, code + 128, under a zero: the f16 subnormals (code + 128) 2^-24, which the MMA takes exactly
+template <uint32_t SEL> __device__ __forceinline__ uint32_t bytes_to_f16(uint32_t x) {
+    return __byte_perm(x, 0u, 0x4040u | (SEL & 0xfu) | ((SEL >> 4) << 8));
+}
+
 template <int HD, bool Q8> struct Smem {
     static constexpr int kRow = HD * (Q8 ? 1 : 2);           // one kv head's part of a cache row
     static constexpr int kTile = kBlock * kRow;
@@ -122,7 +136,7 @@ template <int HD, bool Q8> struct Smem {
     static constexpr int kORow = HD + 4;                     // floats of a head's row in a warp's merge tile
     static constexpr int kMergeTile = kHeads * kORow * 4;
     static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kMisc = 2 * kWarps * kHeads * 4 + kHeads * 4 + 16;
+    static constexpr int kMisc = 2 * kWarps * kHeads * 4 + 2 * kHeads * 4 + 16;
     static constexpr int kTotal = kQ + kRing + kMisc;
     static_assert(kWarps * kMergeTile <= kRing, "the merge tiles reuse the rings");
     static_assert(kMaxSms * kCtas * kHeads * 4 <= kRing, "so do the factors of all records of a unit");
@@ -132,6 +146,7 @@ template <int HD, bool Q8> struct Smem {
 struct Seq {
     uint32_t L, doc, wlo, pre;   // rows; first visible row; first row of the window; prefix rows
     uint32_t a0, na, b0, n;      // prefix blocks a0 .. a0+na-1, then window blocks b0 ..; n in all (at least 1)
+    uint32_t len;                // units on the line per (kv head, group): the blocks and the pad behind them
 };
 __device__ __forceinline__ Seq seq_of(const Args &a, uint32_t s) {
     Seq q;
@@ -146,12 +161,20 @@ __device__ __forceinline__ Seq seq_of(const Args &a, uint32_t s) {
     const uint32_t pe = min(q.pre, q.wlo);
     if (q.doc < pe) q.na = min((pe - 1) / kBlock + 1, nb ? q.b0 : ~0u) - q.a0;   // a block that both parts touch counts as the window's
     q.n = max(1u, q.na + nb);
+    q.len = q.n + a.pad;
     return q;
+}
+// all rows of the block at r0 are seen: inside the window, or inside the prefix
+__device__ __forceinline__ bool whole_block(const Seq &q, uint32_t r0) {
+    return (r0 >= q.wlo && r0 + kBlock <= q.L) || (r0 >= q.doc && r0 + kBlock <= q.pre);
 }
 __device__ __forceinline__ bool visible(const Seq &q, uint32_t row) { return row < q.L && row >= q.doc && (row >= q.wlo || row < q.pre); }
 
+// Where results go, by value: a reference to the kernel's parameters would make a function that is not inlined fetch
+// them through generic memory.
+struct OutRef { void *out; float *lse; float *records; uint32_t nh, out_dtype; };
 // four output elements of a head from the weighted sum o and the sum of the weights l
-template <int HD> __device__ __forceinline__ void put_out(const Args &a, uint32_t seq, uint32_t head, uint32_t d, const float4 &o, float l) {
+template <int HD> __device__ __forceinline__ void put_out(const OutRef &a, uint32_t seq, uint32_t head, uint32_t d, const float4 &o, float l) {
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     const float v[4] = {l > 0.f ? o.x * inv : 0.f, l > 0.f ? o.y * inv : 0.f, l > 0.f ? o.z * inv : 0.f, l > 0.f ? o.w * inv : 0.f};
     const size_t at = ((size_t)seq * a.nh + head) * HD + d;
@@ -159,8 +182,57 @@ template <int HD> __device__ __forceinline__ void put_out(const Args &a, uint32_
     else if (a.out_dtype == SHADY_F16) *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(a.out) + at) = make_uint2(pack<__half>(v[0], v[1]), pack<__half>(v[2], v[3]));
     else *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + at) = make_uint2(pack<__nv_bfloat16>(v[0], v[1]), pack<__nv_bfloat16>(v[2], v[3]));
 }
-__device__ __forceinline__ void put_lse(const Args &a, uint32_t seq, uint32_t head, float m, float l) {
+__device__ __forceinline__ void put_lse(const OutRef &a, uint32_t seq, uint32_t head, float m, float l) {
     if (a.lse) a.lse[(size_t)seq * a.nh + head] = l > 0.f ? (m + log2f(l)) * kRuleLn2 : -INFINITY;
+}
+
+// A CTA joins the records first, first + step, ... (n of them) of a unit into the output, or into record `first`.  Record 0
+// of the unit lies in slot0, record k in slot base + 2k.  sm_w: room for the records' factors [n][kHeads]; sm_l [kHeads].
+// Not inlined: its requests in flight must not cost the streaming loop registers.
+template <int HD>
+__device__ __noinline__ void join(const OutRef a, uint32_t slot0, uint32_t base, uint32_t first, uint32_t step, uint32_t n, uint32_t heads,
+                                  uint32_t seq, uint32_t h0, float *sm_w, float *sm_l, bool to_output) {
+    constexpr int kRec = kHeads * (HD + 2);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto record = [&](uint32_t k) { return a.records + (size_t)(k ? base + 2 * k : slot0) * kRec; };
+    for (uint32_t h = warp; h < heads; h += kWarps) {   // statistics: a warp per head, its lanes take the records
+        float m = -INFINITY, l = 0.f;
+        for (uint32_t k = lane; k < n; k += 32) {
+            const float2 v = __ldcg(reinterpret_cast<const float2 *>(record(first + k * step) + kHeads * HD + 2 * h));
+            sm_w[k * kHeads + h] = v.x;
+            const float mn = fmaxf(m, v.x), mu = mn == -INFINITY ? 0.f : mn;
+            l = l * rule_exp2(m - mu) + v.y * rule_exp2(v.x - mu);
+            m = mn;
+        }
+        const float M = warp_max(m), mu = M == -INFINITY ? 0.f : M;
+        l = warp_sum(l * rule_exp2(m - mu));
+        for (uint32_t k = lane; k < n; k += 32) sm_w[k * kHeads + h] = rule_exp2(sm_w[k * kHeads + h] - mu);
+        if (lane == 0) {
+            sm_l[h] = l;
+            if (to_output) put_lse(a, seq, h0 + h, M, l);
+            else *reinterpret_cast<float2 *>(record(first) + kHeads * HD + 2 * h) = make_float2(M, l);
+        }
+    }
+    __syncthreads();
+    for (uint32_t e = tid; e < heads * (HD / 4); e += kThreads) {
+        const uint32_t h = e / (HD / 4), d = e % (HD / 4) * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr uint32_t kUn = 8;   // records requested together
+        for (uint32_t k0 = 0; k0 < n; k0 += kUn) {
+            float4 v[kUn];
+#pragma unroll
+            for (uint32_t k = 0; k < kUn; ++k)
+                if (k0 + k < n) v[k] = __ldcg(reinterpret_cast<const float4 *>(record(first + (k0 + k) * step) + h * HD + d));
+#pragma unroll
+            for (uint32_t k = 0; k < kUn; ++k)
+                if (k0 + k < n) {
+                    const float f = sm_w[(k0 + k) * kHeads + h];
+                    o.x += f * v[k].x; o.y += f * v[k].y; o.z += f * v[k].z; o.w += f * v[k].w;
+                }
+        }
+        if (to_output) put_out<HD>(a, seq, h0 + h, d, o, sm_l[h]);
+        else *reinterpret_cast<float4 *>(record(first) + h * HD + d) = o;
+    }
 }
 
 template <typename T, int HD, bool Q8>
@@ -172,17 +244,18 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
     constexpr int NI = kBlock / RPI;
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char *sm_q = smem, *sm_ring = smem + S::kQ;
-    float *sm_m = reinterpret_cast<float *>(smem + S::kQ + S::kRing), *sm_l = sm_m + kWarps * kHeads, *sm_qs = sm_l + kWarps * kHeads;
-    uint32_t *sm_flag = reinterpret_cast<uint32_t *>(sm_qs + kHeads);
+    float *sm_m = reinterpret_cast<float *>(smem + S::kQ + S::kRing), *sm_l = sm_m + kWarps * kHeads, *sm_qs = sm_l + kWarps * kHeads, *sm_qsum = sm_qs + kHeads;
+    uint32_t *sm_flag = reinterpret_cast<uint32_t *>(sm_qsum + kHeads);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t g = lane >> 2, t = lane & 3, mat = lane >> 3, rin = lane & 7;
     const uint32_t U = a.nkv * a.groups;
+    const OutRef to{a.out, a.lse, a.records, a.nh, a.out_dtype};
 
     // ---- this CTA's share of the line; every warp works it out for itself ----
     uint32_t total = 0;
     for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += 32) {
         const uint32_t s = s0 + lane;
-        total += __reduce_add_sync(0xffffffffu, s < a.num_seqs ? seq_of(a, s).n * U : 0u);
+        total += __reduce_add_sync(0xffffffffu, s < a.num_seqs ? seq_of(a, s).len * U : 0u);
     }
     const uint32_t share = max((total + gridDim.x - 1) / gridDim.x, kMinShare);
     uint32_t x = blockIdx.x * share;
@@ -191,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
     uint32_t seq = 0, base = 0;   // the sequence that holds x, and where it starts on the line
     for (uint32_t s0 = 0; s0 < a.num_seqs; s0 += 32) {
         const uint32_t s = s0 + lane;
-        const uint32_t n = s < a.num_seqs ? seq_of(a, s).n * U : 0u;
+        const uint32_t n = s < a.num_seqs ? seq_of(a, s).len * U : 0u;
         uint32_t upto = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -212,8 +285,13 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
     const uint32_t q_addr = (uint32_t)__cvta_generic_to_shared(sm_q);
     while (x < x_end) {
         const Seq sq = seq_of(a, seq);
-        const uint32_t unit = (x - base) / sq.n, u0 = base + unit * sq.n, u1 = u0 + sq.n;   // (kv head, head group) on the line
-        const uint32_t p0 = x - u0, p1 = min(x_end, u1) - u0;                               // blocks [p0, p1) of it are this piece
+        const uint32_t unit = (x - base) / sq.len, u0 = base + unit * sq.len, u1 = u0 + sq.n;   // (kv head, head group) on the line
+        auto go_on = [&]() {   // to the next unit, behind this one's pad
+            x = u0 + sq.len;
+            if (unit == U - 1) { base = x; ++seq; }
+        };
+        if (x >= u1) { go_on(); continue; }                    // this share begins in a pad
+        const uint32_t p0 = x - u0, p1 = min(x_end, u1) - u0;   // blocks [p0, p1) of it are this piece
         const bool whole = p1 - p0 == sq.n;
         const uint32_t kvh = unit / a.groups, grp = unit % a.groups;
         const uint32_t heads = min((uint32_t)kHeads, a.G - grp * kHeads);
@@ -248,16 +326,27 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                     row0 = r0;
                 }
             }
-            // a block inside the window or the prefix needs no test per row
-            const bool full = have && ((r0 >= sq.wlo && r0 + kBlock <= sq.L) || (r0 >= sq.doc && r0 + kBlock <= sq.pre));
+            const bool full = have && whole_block(sq, r0);   // no test per row
             const size_t stride = (size_t)a.nkv * S::kRow, off = (size_t)(row0 + l_row) * stride + (size_t)kvh * S::kRow + l_chunk * 16;
+            const uint32_t dst = st + l_row * S::kRow;
+            if (full) {
+                const char *kp = kb + off, *vp = vb + off;
 #pragma unroll
-            for (int k = 0; k < NI; ++k) {
-                const bool ok = full || (have && visible(sq, r0 + k * RPI + l_row));
-                const uint32_t so = (k * RPI + l_row) * S::kRow + ((l_sw ^ S::swz(k * RPI)) << 4);   // swz(a + b) = swz(a) ^ swz(b) here: no common bits
-                const size_t o = ok ? off + (size_t)(k * RPI) * stride : 0;
-                cp16(st + so, kb + o, ok);
-                cp16(st + S::kTile + so, vb + o, ok);
+                for (int k = 0; k < NI; ++k) {
+                    const uint32_t so = k * RPI * S::kRow + ((l_sw ^ S::swz(k * RPI)) << 4);   // swz(a + b) = swz(a) ^ swz(b) here: no common bits
+                    cp16(dst + so, kp, true);
+                    cp16(dst + S::kTile + so, vp, true);
+                    kp += RPI * stride; vp += RPI * stride;
+                }
+            } else {
+#pragma unroll 1
+                for (int k = 0; k < NI; ++k) {
+                    const bool ok = have && visible(sq, r0 + k * RPI + l_row);
+                    const uint32_t so = k * RPI * S::kRow + ((l_sw ^ S::swz(k * RPI)) << 4);
+                    const size_t o = ok ? off + (size_t)(k * RPI) * stride : 0;
+                    cp16(dst + so, kb + o, ok);
+                    cp16(dst + S::kTile + so, vb + o, ok);
+                }
             }
             if constexpr (Q8) {
                 const uint32_t r = lane & 15;
@@ -299,15 +388,22 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                     for (int e = 0; e < E; ++e) v[e] *= down;
                 }
             }
-            if (lane == 0) sm_qs[h] = up;
             unsigned char *rowp = sm_q + h * HD * 2;
+            float sum = 0.f;   // of the elements as the MMA sees them
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
                 const uint32_t d = lane * E + e;
                 uint32_t col = d;   // column (16-bit element) of dim d
                 if constexpr (Q8) col = (d & ~15u) | ((d & 12u) >> 1) | ((d & 2u) << 2);   // 4u, 4u+1 -> 2u, 2u+1; 4u+2, 4u+3 -> 8+2u, ..
-                *reinterpret_cast<uint32_t *>(rowp + (((col >> 3) ^ (h & 7)) << 4) + (col & 7) * 2) = pack<T>(v[e], v[e + 1]);
+                const uint32_t w2 = pack<T>(v[e], v[e + 1]);
+                *reinterpret_cast<uint32_t *>(rowp + (((col >> 3) ^ (h & 7)) << 4) + (col & 7) * 2) = w2;
+                if constexpr (Q8) {
+                    const __half2 h2 = *reinterpret_cast<const __half2 *>(&w2);
+                    sum += __low2float(h2) + __high2float(h2);
+                }
             }
+            if constexpr (Q8) sum = warp_sum(sum);
+            if (lane == 0) { sm_qs[h] = up; sm_qsum[h] = 128.0f * sum; }
         }
         __syncthreads();
         uint32_t qb[HD / 16][2];
@@ -317,10 +413,15 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
             ldm4(r4, q_addr + rin * HD * 2 + (((2 * c + mat) ^ rin) << 4));
             qb[c][0] = r4[0]; qb[c][1] = r4[1]; qb[c + 1][0] = r4[2]; qb[c + 1][1] = r4[3];
         }
-        float zscale[2], slope2[2];   // heads 2t, 2t+1
+        // heads 2t, 2t+1: z = (S - qoff) * ks * zscale; with a cap, zscale leads to the exponent of rule_tanh_of_exp, without
+        // one to z log2(e)
+        float zscale[2], qoff[2], slope2[2];
+        const bool capped = a.rule.cap > 0.f;
+        const float cap2 = a.rule.cap * kRuleLog2e;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            zscale[r] = a.rule.scale * sm_qs[2 * t + r];
+            zscale[r] = a.rule.scale * sm_qs[2 * t + r] * (capped ? a.rule.inv_cap * 2.0f : 1.0f) * kRuleLog2e;
+            qoff[r] = Q8 ? sm_qsum[2 * t + r] : 0.f;
             slope2[r] = a.rule.slopes && 2 * t + r < heads ? __ldg(a.rule.slopes + h0 + 2 * t + r) * kRuleLog2e : 0.f;
         }
 
@@ -346,8 +447,8 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                     ldm4(kb, st + r * S::kRow + ((ch ^ S::swz(r)) << 4));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t ka[4] = {codes_to_f16<0x10>(kb[2 * h]), codes_to_f16<0x10>(kb[2 * h + 1]),
-                                                codes_to_f16<0x32>(kb[2 * h]), codes_to_f16<0x32>(kb[2 * h + 1])};
+                        const uint32_t ka[4] = {bytes_to_f16<0x10>(kb[2 * h]), bytes_to_f16<0x10>(kb[2 * h + 1]),
+                                                bytes_to_f16<0x32>(kb[2 * h]), bytes_to_f16<0x32>(kb[2 * h + 1])};
                         mma<T>(s2[h], ka, qb[c + h][0], qb[c + h][1]);
                     }
                 }
@@ -362,27 +463,27 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
             }
             const float sT[4] = {s2[0][0] + s2[1][0], s2[0][1] + s2[1][1], s2[0][2] + s2[1][2], s2[0][3] + s2[1][3]};
             // ---- the rule; this lane has positions g and g + 8 of heads 2t, 2t+1.  y = z log2(e) (+ log2 vs) ----
+            const bool full = whole_block(sq, r0);
             float y[4], inv_vs[2] = {1.f, 1.f};
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const uint32_t row = r0 + g + 8 * p;
-                const bool ok = visible(sq, row);
                 float ks = 1.f, lvs = 0.f;
                 if constexpr (Q8) {
                     const float *sc = reinterpret_cast<const float *>(sm_ring + warp * ST * S::kStage + (i % ST) * S::kStage + 2 * S::kTile);
                     ks = sc[g + 8 * p];
                     const float vs = fminf(fmaxf(sc[kBlock + g + 8 * p], kRowqScaleMin), kRowqScaleMax);
-                    lvs = __log2f(vs);
-                    inv_vs[p] = 1.0f / vs;
+                    lvs = rule_log2(vs);
+                    inv_vs[p] = rule_rcp(vs);
                 }
                 const float dist = (float)(sq.L - 1 - row);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    float z = sT[2 * p + r] * ks * zscale[r];
-                    if (a.rule.cap > 0.f) z = a.rule.cap * rule_tanh_of_exp(z * a.rule.inv_cap * (2.0f * kRuleLog2e));
-                    const float v = z * kRuleLog2e - slope2[r] * dist + lvs;
-                    y[2 * p + r] = ok ? v : -INFINITY;
+                    float z = Q8 ? fmaf(sT[2 * p + r], 16777216.0f, -qoff[r]) * ks * zscale[r] : sT[2 * p + r] * zscale[r];
+                    if (capped) z = cap2 * rule_tanh_of_exp(z);
+                    y[2 * p + r] = fmaf(-slope2[r], dist, z) + lvs;
                 }
+                if (!full && !visible(sq, row)) y[2 * p] = y[2 * p + 1] = -INFINITY;
             }
             float corr[2], pw[4];
 #pragma unroll
@@ -469,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
             }
             sm_l[tid] = l;
             if (whole) {
-                if (tid < heads) put_lse(a, seq, h0 + tid, m, l);
+                if (tid < heads) put_lse(to, seq, h0 + tid, m, l);
             } else {
                 *reinterpret_cast<float2 *>(rec + kHeads * HD + 2 * tid) = make_float2(m, l);
             }
@@ -484,65 +585,42 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                 const float4 v = *reinterpret_cast<const float4 *>(sm_ring + w * S::kMergeTile + (h * S::kORow + d) * 4);
                 o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
             }
-            if (whole) put_out<HD>(a, seq, h0 + h, d, o, sm_l[h]);
+            if (whole) put_out<HD>(to, seq, h0 + h, d, o, sm_l[h]);
             else *reinterpret_cast<float4 *>(rec + h * HD + d) = o;
         }
         if (!whole) {
-            // ---- the last CTA to arrive joins the records of this (sequence, kv head, group) ----
+            // ---- the last CTA to arrive joins the records of this (sequence, kv head, group); more than kFlat of them in
+            //      two steps, groups of kFan first, so that no CTA walks a long list while the others idle ----
             const uint32_t c0 = u0 / share, c1 = (u1 - 1) / share, nrec = c1 - c0 + 1;
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) *sm_flag = atomicAdd(a.counters + (size_t)seq * U + unit, 1u);
-            __syncthreads();
-            if (*sm_flag == nrec - 1) {
+            // share c0 wrote the piece as its last one (slot 1) unless the piece began with the share
+            auto slot_of = [&](uint32_t k) { return k ? 2 * (c0 + k) : 2 * c0 + (u0 == c0 * share ? 0u : 1u); };
+            auto arrive_last = [&](uint32_t *counter, uint32_t n) {   // all threads: whether this CTA is the n-th; it then leaves the counter at zero
                 __threadfence();
-                if (tid == 0) a.counters[(size_t)seq * U + unit] = 0;
-                // share c0 wrote the piece as its last one (slot 1) unless the piece began with the share
-                const uint32_t slot0 = 2 * c0 + (u0 == c0 * share ? 0u : 1u);
-                auto record = [&](uint32_t k) { return a.records + (size_t)(k ? 2 * (c0 + k) : slot0) * kRec; };
-                float *sm_w = reinterpret_cast<float *>(sm_ring);   // the records' factors [nrec][kHeads]
-                // a warp finds the statistics of two heads: its lanes take the records
-                for (uint32_t h = warp; h < heads; h += kWarps) {
-                    float m = -INFINITY, l = 0.f;
-                    for (uint32_t k = lane; k < nrec; k += 32) {
-                        const float v = __ldcg(record(k) + kHeads * HD + 2 * h);
-                        sm_w[k * kHeads + h] = v;
-                        m = fmaxf(m, v);
-                    }
-                    m = warp_max(m);
-                    const float mu = m == -INFINITY ? 0.f : m;
-                    for (uint32_t k = lane; k < nrec; k += 32) {
-                        const float f = rule_exp2(sm_w[k * kHeads + h] - mu);
-                        sm_w[k * kHeads + h] = f;
-                        l += f * __ldcg(record(k) + kHeads * HD + 2 * h + 1);
-                    }
-                    l = warp_sum(l);
-                    if (lane == 0) { sm_l[h] = l; put_lse(a, seq, h0 + h, m, l); }
-                }
                 __syncthreads();
-                for (uint32_t e = tid; e < heads * (HD / 4); e += kThreads) {
-                    const uint32_t h = e / (HD / 4), d = e % (HD / 4) * 4;
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                    constexpr uint32_t kUn = 16;   // records requested together
-                    for (uint32_t k0 = 0; k0 < nrec; k0 += kUn) {
-                        float4 v[kUn];
-#pragma unroll
-                        for (uint32_t k = 0; k < kUn; ++k)
-                            if (k0 + k < nrec) v[k] = __ldcg(reinterpret_cast<const float4 *>(record(k0 + k) + h * HD + d));
-#pragma unroll
-                        for (uint32_t k = 0; k < kUn; ++k)
-                            if (k0 + k < nrec) {
-                                const float f = sm_w[(k0 + k) * kHeads + h];
-                                o.x += f * v[k].x; o.y += f * v[k].y; o.z += f * v[k].z; o.w += f * v[k].w;
-                            }
-                    }
-                    put_out<HD>(a, seq, h0 + h, d, o, sm_l[h]);
+                if (tid == 0) *sm_flag = atomicAdd(counter, 1u);
+                __syncthreads();
+                const bool last = *sm_flag == n - 1;
+                if (last) {
+                    __threadfence();
+                    if (tid == 0) *counter = 0;
+                }
+                return last;
+            };
+            float *sm_w = reinterpret_cast<float *>(sm_ring);
+            uint32_t *unit_counter = a.counters + (size_t)seq * U + unit;
+            if (nrec <= kFlat) {
+                if (arrive_last(unit_counter, nrec)) join<HD>(to, slot_of(0), 2 * c0, 0, 1, nrec, heads, seq, h0, sm_w, sm_l, true);
+            } else {
+                const uint32_t first = (blockIdx.x - c0) / kFan * kFan, n = min(kFan, nrec - first);
+                if (arrive_last(a.group_counters + slot_of(first), n)) {
+                    join<HD>(to, slot_of(0), 2 * c0, first, 1, n, heads, seq, h0, sm_w, sm_l, false);
+                    const uint32_t groups = (nrec + kFan - 1) / kFan;
+                    if (arrive_last(unit_counter, groups)) join<HD>(to, slot_of(0), 2 * c0, 0, kFan, groups, heads, seq, h0, sm_w, sm_l, true);
                 }
             }
         }
         __syncthreads();   // the rings and the statistics are free for the next piece
-        x = u0 + p1;
-        if (x >= u1 && unit == U - 1) { base = u1; ++seq; }
+        go_on();   // (a piece that ends with the share, not with its unit, leaves x behind x_end: done)
     }
 }
 
@@ -560,11 +638,12 @@ static int check(shady_ctx *ctx, const shady_decode_params *p) {
     return SHADY_OK;
 }
 constexpr uint32_t kMaxCtasPerSm = 3;
-static size_t counter_bytes(const shady_decode_params *p) {
-    return ((size_t)p->num_seqs * p->num_kv_heads * head_groups(p) * 4 + 255) & ~(size_t)255;
+static size_t group_words(const shady_ctx *ctx) { return (size_t)2 * ctx->num_sms * kMaxCtasPerSm; }
+static size_t counter_bytes(const shady_ctx *ctx, const shady_decode_params *p) {
+    return (((size_t)p->num_seqs * p->num_kv_heads * head_groups(p) + group_words(ctx)) * 4 + 255) & ~(size_t)255;
 }
 static size_t workspace_bytes(const shady_ctx *ctx, const shady_decode_params *p) {
-    return counter_bytes(p) + (size_t)2 * ctx->num_sms * kMaxCtasPerSm * kHeads * (p->head_dim + 2) * 4;
+    return counter_bytes(ctx, p) + (size_t)2 * ctx->num_sms * kMaxCtasPerSm * kHeads * (p->head_dim + 2) * 4;
 }
 
 template <typename T, int HD, bool Q8> static int launch(shady_ctx *ctx, const Args &a) {
@@ -589,7 +668,7 @@ int decode_rule_workspace_size(shady_ctx *ctx, const shady_decode_params *p, siz
 int decode_rule_workspace_init(shady_ctx *ctx, const shady_decode_params *p, void *d_ws, size_t ws_bytes) {
     if (const int st = dr::check(ctx, p)) return st;
     SHADY_REQUIRE(ctx, d_ws && ws_bytes >= dr::workspace_bytes(ctx, p), SHADY_ERR_WORKSPACE, "decode_rule: workspace missing or too small");
-    SHADY_CUDA_OK(ctx, cudaMemsetAsync(d_ws, 0, dr::counter_bytes(p), ctx->stream));
+    SHADY_CUDA_OK(ctx, cudaMemsetAsync(d_ws, 0, dr::counter_bytes(ctx, p), ctx->stream));
     return SHADY_OK;
 }
 
@@ -614,10 +693,12 @@ int launch_decode_rule(shady_ctx *ctx, const shady_decode_params *p, const shady
     SHADY_REQUIRE(ctx, d_ws && ((uintptr_t)d_ws & 15) == 0 && ws_bytes >= dr::workspace_bytes(ctx, p), SHADY_ERR_WORKSPACE,
                   "decode_rule: workspace missing, unaligned or too small");
     a.q = d_q; a.out = d_out; a.lse = d_lse; a.lens = d_seq_lens;
-    a.counters = reinterpret_cast<uint32_t *>(d_ws);
-    a.records = reinterpret_cast<float *>(reinterpret_cast<char *>(d_ws) + dr::counter_bytes(p));
+    a.group_counters = reinterpret_cast<uint32_t *>(d_ws);
+    a.counters = a.group_counters + dr::group_words(ctx);
+    a.records = reinterpret_cast<float *>(reinterpret_cast<char *>(d_ws) + dr::counter_bytes(ctx, p));
     a.num_seqs = p->num_seqs; a.nkv = p->num_kv_heads; a.nh = p->num_q_heads; a.G = a.nh / a.nkv; a.groups = dr::head_groups(p);
     a.q_dtype = p->q_dtype; a.out_dtype = p->out_dtype;
+    a.pad = dr::kPad;
     auto by_dim = [&](auto t, auto q8) {
         using T = decltype(t);
         constexpr bool Q8 = decltype(q8)::value;

@@ -30,6 +30,11 @@ __device__ __forceinline__ float rule_rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float rule_log2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // tanh(z) = 1 - 2 / (1 + e^(2z)), with z2 = 2 z log2(e).  The absolute error is a few 2^-24 everywhere (near 0 the
 // two halves cancel, but a score needs cap * tanh to an absolute error, not a relative one); tanh.approx is 2^-11 off,
 // which a cap of 50 turns into 2 % of a weight.
