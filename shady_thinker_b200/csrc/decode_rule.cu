@@ -110,6 +110,12 @@ template <typename T> __device__ __forceinline__ uint32_t pack(float lo, float h
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
+// N consecutive elements (2, 4 or 8) as f32, one or two accesses
+template <typename T, int N> __device__ __forceinline__ void vec_load(const T *p, float (&v)[N]) {
+    struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Raw { T e[N]; } raw = *reinterpret_cast<const Raw *>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = to_f32<T>(raw.e[i]);
+}
 // bytes SEL & 0xf and SEL >> 4 of x, each a code + 128, as the f16 pair of the codes
 template <uint32_t SEL> __device__ __forceinline__ uint32_t codes_to_f16(uint32_t x) {
     const uint32_t w = __byte_perm(x, 0x64646464u, 0x4040u | (SEL & 0xfu) | ((SEL >> 4) << 8));
@@ -128,9 +134,11 @@ template <int HD, bool Q8> struct Smem {
     // 16-byte chunk c of row r lies in place c ^ swz(r): the eight rows of an ldmatrix then fall on different banks
     static __device__ __forceinline__ uint32_t swz(uint32_t r) { return kRow >= 128 ? r & 7 : (r >> 1) & 3; }
     static constexpr int kScales = Q8 ? 2 * kBlock * 4 : 0;  // the block's K scales, then its V scales
-    static constexpr int kStage = 2 * kTile + kScales;
-    // stages of a warp's ring: with the CTAs an SM then holds (kCtas), 96..192 KB of an SM's rows are in flight
-    static constexpr int kStages = kStage >= 16384 ? 3 : (kStage >= 8192 ? 3 : 4);
+    static constexpr int kStage = 2 * kTile + kScales;       // one block
+    // With the CTAs an SM then holds (kCtas), two blocks of each of its warps are in flight, 100..130 KB an SM.  Measured
+    // against it on the ragged row-scaled batch (43.0 us): four stages 43.7, four CTAs of at most 128 registers 47.0, two
+    // blocks per step of half the warps 48.1.
+    static constexpr int kStages = 3;
     static constexpr int kCtas = kStage >= 16384 ? 1 : (kStage >= 8192 ? 2 : 3);
     static constexpr int kQ = kHeads * HD * 2;
     static constexpr int kORow = HD + 4;                     // floats of a head's row in a warp's merge tile
@@ -248,6 +256,10 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
     uint32_t *sm_flag = reinterpret_cast<uint32_t *>(sm_qsum + kHeads);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t g = lane >> 2, t = lane & 3, mat = lane >> 3, rin = lane & 7;
+    // a launch in programmatic stream order starts while the kernel before it drains; nothing that kernel may have written is
+    // read before it has completed
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t U = a.nkv * a.groups;
     const OutRef to{a.out, a.lse, a.records, a.nh, a.out_dtype};
 
@@ -296,65 +308,80 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
         const uint32_t kvh = unit / a.groups, grp = unit % a.groups;
         const uint32_t heads = min((uint32_t)kHeads, a.G - grp * kHeads);
         const uint32_t h0 = kvh * a.G + grp * kHeads;   // first query head
-        const uint32_t my_n = p1 - p0 > warp ? (p1 - p0 - warp + kWarps - 1) / kWarps : 0;
+        const uint32_t my_n = p1 - p0 > warp ? (p1 - p0 - warp + kWarps - 1) / kWarps : 0;   // this warp's blocks
 
-        const char *kbase = nullptr, *vbase = nullptr;
-        if constexpr (!Q8) {
-            if (a.kv.page_table) { kbase = a.kv.k_base; vbase = a.kv.v_base; }
-            else {
-                kbase = kv_seq_ptr(a.kv.k_base, a.kv.k_ptrs, a.kv.seq_stride_bytes, seq);
-                vbase = kv_seq_ptr(a.kv.v_base, a.kv.v_ptrs, a.kv.seq_stride_bytes, seq);
-            }
-        }
-        auto row_of_block = [&](uint32_t b) { return (b < sq.na ? sq.a0 + b : sq.b0 + (b - sq.na)) * kBlock; };
+        // this lane's part of the first row of the sequence's cache, or of the pools' first page
         const uint32_t l_row = lane / CH % RPI, l_chunk = lane % CH, l_sw = l_chunk ^ S::swz(l_row);
-        // row numbers of the caches are taken relative to a base that the block's page or sequence gives
+        const uint32_t stride = a.nkv * S::kRow;   // bytes of a cache row
+        const bool paged = Q8 ? a.rq.page_table != nullptr : a.kv.page_table != nullptr;
+        const uint32_t page_rows = Q8 ? a.rq.page_rows : a.kv.page_rows, max_pages = Q8 ? a.rq.max_pages : a.kv.max_pages;
+        const uint32_t *table = paged ? (Q8 ? a.rq.page_table : a.kv.page_table) + (size_t)seq * max_pages : nullptr;
+        const uint32_t cap = Q8 && !paged ? (uint32_t)min(a.rq.seq_rows, 0xffffffffull) : 0xffffffffu;
+        const char *kbase, *vbase;
+        size_t s_off = 0;   // the sequence's first scale
+        if constexpr (Q8) {
+            const size_t first = paged ? 0 : (size_t)seq * a.rq.seq_rows;
+            kbase = reinterpret_cast<const char *>(a.rq.k_codes) + first * stride;
+            vbase = reinterpret_cast<const char *>(a.rq.v_codes) + first * stride;
+            s_off = first * a.nkv;
+        } else {
+            kbase = paged ? a.kv.k_base : kv_seq_ptr(a.kv.k_base, a.kv.k_ptrs, a.kv.seq_stride_bytes, seq);
+            vbase = paged ? a.kv.v_base : kv_seq_ptr(a.kv.v_base, a.kv.v_ptrs, a.kv.seq_stride_bytes, seq);
+        }
+        auto row_of = [&](uint32_t i) {   // first row of this warp's i-th block
+            const uint32_t b = p0 + warp + i * kWarps;
+            return (b < sq.na ? sq.a0 + b : sq.b0 + (b - sq.na)) * kBlock;
+        };
+        // The page of a block is asked for a block before its rows are; a block without a visible row asks for none, so the
+        // table is only read where the sequence owns the page.
+        constexpr uint32_t kNoPage = 0xffffffffu;
+        uint32_t page = kNoPage;
+        auto ask_page = [&](uint32_t i) {
+            page = kNoPage;
+            if (!paged || i >= my_n) return;
+            const uint32_t r0 = row_of(i);
+            if (r0 < sq.L && r0 + kBlock > sq.doc && r0 / page_rows < max_pages) page = __ldg(table + r0 / page_rows);
+        };
         auto issue = [&](uint32_t i) {
-            const uint32_t r0 = row_of_block(p0 + warp + i * kWarps);
-            const uint32_t st = ring + (i % ST) * S::kStage;
-            bool have = r0 < sq.L && r0 + kBlock > sq.doc;   // some row of the block is visible: its page is the sequence's own
-            unsigned long long row0 = 0;                     // first row of the block, counted in whole cache rows
-            const char *kb = kbase, *vb = vbase;
-            if (have) {
-                if constexpr (Q8) {
-                    have = rowq_row(a.rq, seq, r0, row0);
-                    kb = reinterpret_cast<const char *>(a.rq.k_codes); vb = reinterpret_cast<const char *>(a.rq.v_codes);
-                } else if (a.kv.page_table) {
-                    have = r0 / a.kv.page_rows < a.kv.max_pages;
-                    if (have) row0 = (unsigned long long)__ldg(a.kv.page_table + (size_t)seq * a.kv.max_pages + r0 / a.kv.page_rows) * a.kv.page_rows + r0 % a.kv.page_rows;
-                } else {
-                    row0 = r0;
-                }
+            const uint32_t r0 = row_of(i), st = ring + (i % ST) * S::kStage;
+            size_t row0 = r0;            // first row of the block, counted from the base
+            bool have = r0 < cap;
+            if (paged) {
+                have = page != kNoPage && !(Q8 && a.rq.num_pages && page >= a.rq.num_pages);
+                row0 = (size_t)page * page_rows + r0 % page_rows;
             }
-            const bool full = have && whole_block(sq, r0);   // no test per row
-            const size_t stride = (size_t)a.nkv * S::kRow, off = (size_t)(row0 + l_row) * stride + (size_t)kvh * S::kRow + l_chunk * 16;
+            const bool full = have && whole_block(sq, r0) && r0 + kBlock <= cap;   // no test per row
+            const size_t off = (row0 + l_row) * stride + (size_t)kvh * S::kRow + l_chunk * 16;
             const uint32_t dst = st + l_row * S::kRow;
             if (full) {
-                const char *kp = kb + off, *vp = vb + off;
+                const char *kp = kbase + off, *vp = vbase + off;
 #pragma unroll
                 for (int k = 0; k < NI; ++k) {
                     const uint32_t so = k * RPI * S::kRow + ((l_sw ^ S::swz(k * RPI)) << 4);   // swz(a + b) = swz(a) ^ swz(b) here: no common bits
                     cp16(dst + so, kp, true);
                     cp16(dst + S::kTile + so, vp, true);
-                    kp += RPI * stride; vp += RPI * stride;
+                    kp += (size_t)RPI * stride; vp += (size_t)RPI * stride;
                 }
             } else {
 #pragma unroll 1
                 for (int k = 0; k < NI; ++k) {
-                    const bool ok = have && visible(sq, r0 + k * RPI + l_row);
+                    const uint32_t row = r0 + k * RPI + l_row;
+                    const bool ok = have && visible(sq, row) && row < cap;
                     const uint32_t so = k * RPI * S::kRow + ((l_sw ^ S::swz(k * RPI)) << 4);
                     const size_t o = ok ? off + (size_t)(k * RPI) * stride : 0;
-                    cp16(dst + so, kb + o, ok);
-                    cp16(dst + S::kTile + so, vb + o, ok);
+                    cp16(dst + so, kbase + o, ok);
+                    cp16(dst + S::kTile + so, vbase + o, ok);
                 }
             }
             if constexpr (Q8) {
                 const uint32_t r = lane & 15;
-                const bool ok = full || (have && visible(sq, r0 + r));
-                const float *sc = lane < 16 ? a.rq.k_scales : a.rq.v_scales;
-                cp4(st + 2 * S::kTile + lane * 4, sc + (ok ? (size_t)(row0 + r) * a.nkv + kvh : 0), ok);
+                const bool ok = full || (have && visible(sq, r0 + r) && r0 + r < cap);
+                const float *sc = (lane < 16 ? a.rq.k_scales : a.rq.v_scales) + s_off + kvh;
+                cp4(st + 2 * S::kTile + lane * 4, sc + (ok ? (row0 + r) * a.nkv : 0), ok);
             }
+            ask_page(i + 1);
         };
+        ask_page(0);
 #pragma unroll
         for (int i = 0; i < ST - 1; ++i) {
             if ((uint32_t)i < my_n) issue(i);
@@ -370,8 +397,9 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
             for (int e = 0; e < E; ++e) v[e] = 0.f;
             if (h < heads) {
                 const size_t o = ((size_t)seq * a.nh + h0 + h) * HD + lane * E;
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = load_as_f32(a.q, o + e, a.q_dtype);
+                if (a.q_dtype == SHADY_F32) vec_load<float, E>(reinterpret_cast<const float *>(a.q) + o, v);
+                else if (a.q_dtype == SHADY_F16) vec_load<__half, E>(reinterpret_cast<const __half *>(a.q) + o, v);
+                else vec_load<__nv_bfloat16, E>(reinterpret_cast<const __nv_bfloat16 *>(a.q) + o, v);
             }
             float up = 1.f;
             if constexpr (Q8) {
@@ -436,9 +464,8 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
             if (i + ST - 1 < my_n) issue(i + ST - 1);
             cp_commit();
             const uint32_t st = ring + (i % ST) * S::kStage;
-            const uint32_t r0 = row_of_block(p0 + warp + i * kWarps);
-            // ---- S^T: 16 positions x 8 heads ----
-            float s2[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};   // two chains of products: half the dependent MMAs
+            // ---- S^T: 16 positions x 8 heads, in two chains of products ----
+            float s2[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
             if constexpr (Q8) {
 #pragma unroll
                 for (int c = 0; c < CH; c += 2) {
@@ -461,8 +488,8 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                     mma<T>(s2[c & 1], ka, qb[c][0], qb[c][1]);
                 }
             }
-            const float sT[4] = {s2[0][0] + s2[1][0], s2[0][1] + s2[1][1], s2[0][2] + s2[1][2], s2[0][3] + s2[1][3]};
             // ---- the rule; this lane has positions g and g + 8 of heads 2t, 2t+1.  y = z log2(e) (+ log2 vs) ----
+            const uint32_t r0 = row_of(i);
             const bool full = whole_block(sq, r0);
             float y[4], inv_vs[2] = {1.f, 1.f};
 #pragma unroll
@@ -470,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                 const uint32_t row = r0 + g + 8 * p;
                 float ks = 1.f, lvs = 0.f;
                 if constexpr (Q8) {
-                    const float *sc = reinterpret_cast<const float *>(sm_ring + warp * ST * S::kStage + (i % ST) * S::kStage + 2 * S::kTile);
+                    const float *sc = reinterpret_cast<const float *>(sm_ring + (warp * ST + i % ST) * S::kStage + 2 * S::kTile);
                     ks = sc[g + 8 * p];
                     const float vs = fminf(fmaxf(sc[kBlock + g + 8 * p], kRowqScaleMin), kRowqScaleMax);
                     lvs = rule_log2(vs);
@@ -479,7 +506,8 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
                 const float dist = (float)(sq.L - 1 - row);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    float z = Q8 ? fmaf(sT[2 * p + r], 16777216.0f, -qoff[r]) * ks * zscale[r] : sT[2 * p + r] * zscale[r];
+                    const float sT = s2[0][2 * p + r] + s2[1][2 * p + r];
+                    float z = Q8 ? fmaf(sT, 16777216.0f, -qoff[r]) * ks * zscale[r] : sT * zscale[r];
                     if (capped) z = cap2 * rule_tanh_of_exp(z);
                     y[2 * p + r] = fmaf(-slope2[r], dist, z) + lvs;
                 }
@@ -651,7 +679,17 @@ template <typename T, int HD, bool Q8> static int launch(shady_ctx *ctx, const A
     static_assert(S::kCtas <= (int)kMaxCtasPerSm && S::kCtas * (S::kTotal + 1024) <= 228 * 1024, "resident CTAs");
     auto kern = decode_rule_kernel<T, HD, Q8>;
     SHADY_CUDA_OK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal));
-    kern<<<ctx->num_sms * S::kCtas, kThreads, S::kTotal, ctx->stream>>>(a);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctx->num_sms * S::kCtas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = S::kTotal;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    SHADY_CUDA_OK(ctx, cudaLaunchKernelEx(&cfg, kern, a));
     ctx->launches++;
     SHADY_CUDA_OK(ctx, cudaGetLastError());
     return SHADY_OK;
