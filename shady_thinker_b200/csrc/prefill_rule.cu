@@ -96,6 +96,43 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
                  ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
 }
 
+__device__ __forceinline__ unsigned long long mul_f32x2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long both(float v) { return pack_f32x2(v, v); }
+// Two raw products s -> cap tanh(s scale / cap) log2(e), with c = scale / cap and scale2 = scale log2(e), for |s c| <=
+// kTanhSmall: a polynomial on the FMA pipe, no special function.  Scores within the cap are the common case: the 4 x 4096
+// batch takes 0.69 ms where exponential and reciprocal per element take 1.06 and a quotient of polynomials for all
+// arguments 1.32.
+__device__ __forceinline__ void cap_small(uint32_t &s0, uint32_t &s1, float c, float scale2) {
+    const unsigned long long s = pack_f32x2(__uint_as_float(s0), __uint_as_float(s1));
+    const unsigned long long x = mul_f32x2(s, both(c)), t = mul_f32x2(x, x);
+    unsigned long long p = fma2(t, both(kTanhC5), both(kTanhC4));
+    p = fma2(p, t, both(kTanhC3));
+    p = fma2(p, t, both(kTanhC2));
+    p = fma2(p, t, both(kTanhC1));
+    p = fma2(p, t, both(kTanhC0));
+    p = mul_f32x2(p, mul_f32x2(s, both(scale2)));   // cap2 x = s scale2
+    float y0, y1;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(p));
+    s0 = __float_as_uint(y0); s1 = __float_as_uint(y1);
+}
+// The same for all arguments: 1 - 2 / (1 + e^(2x)), one reciprocal for two elements; at an exponent of 60 the tanh is 1 to
+// the last bit, and the product of two sums still fits f32.
+__device__ __forceinline__ void cap_any(uint32_t &s0, uint32_t &s1, float c, float cap2) {
+    const float ci = c * (2.0f * kRuleLog2e);
+    const float e0 = 1.0f + rule_exp2(fminf(__uint_as_float(s0) * ci, 60.f)), e1 = 1.0f + rule_exp2(fminf(__uint_as_float(s1) * ci, 60.f));
+    const float r = rule_rcp(e0 * e1) * (-2.0f * cap2);
+    s0 = __float_as_uint(fmaf(r, e1, cap2)); s1 = __float_as_uint(fmaf(r, e0, cap2));
+}
+
 // MODE 0: scale only, 1: tanh cap, 2: distance bias, with or without a cap
 template <typename T, int HD, int MODE>
 __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
@@ -156,64 +193,83 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == kWSched) {
         // =============================== items ===============================
-        uint32_t chunk = 0, base = 0, upto = 0, mine = 0, all = 0, ic = 0;   // 32 sequences at a time, one per lane
-        uint32_t qs = 0, T_s = 0;
+        // 32 sequences at a time, one per lane.  A sequence's blocks stand at levels [lo, hi) = their first position / TPI; the
+        // list runs from the highest level down (the blocks with the most rows in front of them first, so that the list
+        // ends with small items), at one level over the sequences that have a block there, for each over the kv heads.
+        uint32_t chunk = 0, ic = 0;
+        uint32_t qs = 0, T_s = 0, lo = 0, hi = 0;
+        unsigned long long base = 0, w = 0;   // items in front of `level`; the item wanted
+        uint32_t level = 0;                   // levels above it are done; 0: none left in this chunk
         auto load_chunk = [&]() {
             const uint32_t s = chunk + lane;
-            qs = T_s = 0;
+            qs = T_s = lo = hi = 0;
             if (s < a.num_seqs) {
                 qs = min(__ldg(a.q_starts + s), a.total_q);
                 T_s = max(min(__ldg(a.q_starts + s + 1), a.total_q), qs) - qs;
+                const uint32_t L = __ldg(a.kv_lens + s);
+                lo = L > T_s ? (L - T_s) / TPI : 0u;
+                hi = lo + (T_s + TPI - 1) / TPI;
             }
-            mine = (T_s + TPI - 1) / TPI * a.nkv;
-            upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= (uint32_t)o) upto += v;
-            }
-            all = __shfl_sync(0xffffffffu, upto, 31);
+            level = __reduce_max_sync(0xffffffffu, T_s ? hi : 0u);
         };
         load_chunk();
         bool ok = true, more = true;
         for (uint32_t rnd = 0; more && ok; ++rnd, ++ic) {
-            const uint32_t w = rnd * gridDim.x + ((rnd & 1u) ? gridDim.x - 1u - blockIdx.x : blockIdx.x);
-            while (w >= base + all) {
-                if (chunk + 32 >= a.num_seqs) { more = false; break; }
-                base += all; chunk += 32;
-                load_chunk();
+            w = (unsigned long long)rnd * gridDim.x + ((rnd & 1u) ? gridDim.x - 1u - blockIdx.x : blockIdx.x);
+            uint32_t active = 0;   // sequences with a block at level - 1
+            while (true) {
+                if (!level) {
+                    if (chunk + 32 >= a.num_seqs) { more = false; break; }
+                    chunk += 32;
+                    load_chunk();
+                    continue;
+                }
+                // the active set stays the same from level - 1 down to `stay`
+                const uint32_t top = level - 1;
+                active = __ballot_sync(0xffffffffu, lo <= top && top < hi);
+                const uint32_t stay = __reduce_max_sync(0xffffffffu, hi <= top ? hi : (lo <= top ? lo : 0u));
+                const unsigned long long per = (unsigned long long)__popc(active) * a.nkv;
+                if (!per) { level = stay; continue; }   // (stay <= top: a gap between the sequences' levels)
+                const unsigned long long skip = (w - base) / per;
+                if (skip < (unsigned long long)(level - stay)) {
+                    base += skip * per; level -= (uint32_t)skip;
+                    break;
+                }
+                base += (unsigned long long)(level - stay) * per;
+                level = stay;
             }
             uint32_t vals[13] = {0};
             if (more) {
-                const uint32_t k = __ffs(__ballot_sync(0xffffffffu, w < base + upto)) - 1;
-                const uint32_t seq = chunk + k, rem = w - base - __shfl_sync(0xffffffffu, upto - mine, k);
+                const uint32_t rem = (uint32_t)(w - base), nth = rem / a.nkv, kvh = rem % a.nkv;
+                const bool mine = ((active >> lane) & 1u) && (uint32_t)__popc(active & ((1u << lane) - 1u)) == nth;
+                const uint32_t k = __ffs(__ballot_sync(0xffffffffu, mine)) - 1, seq = chunk + k;
                 const uint32_t q0 = __shfl_sync(0xffffffffu, qs, k), len = __shfl_sync(0xffffffffu, T_s, k);
-                const uint32_t blk = (len + TPI - 1) / TPI - 1 - rem / a.nkv;
+                const uint32_t blk = level - 1 - __shfl_sync(0xffffffffu, lo, k);
                 const uint32_t tok0 = q0 + blk * TPI, ntok = min(TPI, len - blk * TPI);
                 const uint32_t L = min(__ldg(a.kv_lens + seq), 0x7fffff00u);
                 const int32_t pos0 = (int32_t)L - (int32_t)len + (int32_t)(blk * TPI), p_hi = pos0 + (int32_t)ntok - 1;
-                uint32_t lo = 0;   // first row that a token of the item may see
+                uint32_t first = 0;   // first row that a token of the item may see
                 if (a.rule.doc) {
-                    lo = 0xffffffffu;
+                    first = 0xffffffffu;
                     for (uint32_t t = lane; t < ntok; t += 32) {
                         const uint32_t d = __ldg(a.rule.doc + tok0 + t);
-                        if (pos0 + (int32_t)t >= 0) lo = min(lo, d);
+                        if (pos0 + (int32_t)t >= 0) first = min(first, d);
                     }
-                    lo = __reduce_min_sync(0xffffffffu, lo);
+                    first = __reduce_min_sync(0xffffffffu, first);
                 }
                 const uint32_t pre = a.rule.prefix ? min(__ldg(a.rule.prefix + seq), L) : 0u;
                 const uint32_t p_lo = (uint32_t)max(pos0, 0);
                 uint32_t a0 = 0, na = 0, b0 = 0, n = 0;
-                if (p_hi >= 0 && lo < L) {
-                    const uint32_t wlo = max(lo, a.rule.window && p_lo + 1 > a.rule.window ? p_lo + 1 - a.rule.window : 0u);
+                if (p_hi >= 0 && first < L) {
+                    const uint32_t wlo = max(first, a.rule.window && p_lo + 1 > a.rule.window ? p_lo + 1 - a.rule.window : 0u);
                     const uint32_t tb0 = wlo / N, tb1 = wlo <= (uint32_t)p_hi ? (uint32_t)p_hi / N + 1 : tb0;
-                    const uint32_t ta0 = lo / N, ta1 = lo < pre ? (pre - 1) / N + 1 : ta0;
+                    const uint32_t ta0 = first / N, ta1 = first < pre ? (pre - 1) / N + 1 : ta0;
                     if (ta1 == ta0) { b0 = tb0; n = tb1 - tb0; }
                     else if (tb1 == tb0 || ta1 >= tb0) { b0 = ta0; n = max(ta1, tb1) - ta0; }
                     else { a0 = ta0; na = ta1 - ta0; b0 = tb0; n = na + tb1 - tb0; }
                 }
                 const uint32_t row0 = a.kv_starts ? __ldg(a.kv_starts + seq) : (uint32_t)min(seq * a.seq_rows, 0x7fffff00ull);
-                const uint32_t v[13] = {1u, seq, rem % a.nkv, tok0, ntok, (uint32_t)pos0, L, row0, a0, na, b0, n, pre};
+                const uint32_t v[13] = {1u, seq, kvh, tok0, ntok, (uint32_t)pos0, L, row0, a0, na, b0, n, pre};
 #pragma unroll
                 for (int i = 0; i < 13; ++i) vals[i] = v[i];
             }
@@ -426,7 +482,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const uint32_t t_o = t_lane + C::kColO + q * 128;
         const uint32_t t_rel = q * TPT + r / a.G, g = r % a.G;
         const float scale2 = a.rule.scale * kRuleLog2e;
-        const float cap_in = a.rule.scale * a.rule.inv_cap * (2.0f * kRuleLog2e), cap2 = a.rule.cap * kRuleLog2e;
+        const float cap_c = a.rule.scale * a.rule.inv_cap, cap2 = a.rule.cap * kRuleLog2e;
         bool ok = true;
         uint32_t cnt = 0, oc = 0;   // score tiles and items of this row tile so far (barrier phases)
         Item it{};
@@ -459,26 +515,49 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const bool whole = !live || (c_lo <= k0 && c_hi >= k0 + (int32_t)N) || (p_lo <= k0 && p_hi >= k0 + (int32_t)N);
                 tmem_wait_ld();
                 // ---- the rule: x = z log2(e), or with scale alone the raw product ----
-                if (MODE != 0) {
+                if (MODE == 1 || (MODE == 2 && a.rule.cap > 0.f)) {
+                    float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (uint32_t c = 0; c < N / 32; ++c)
 #pragma unroll
-                        for (uint32_t i = 0; i < 32; i += 2) {
-                            float y0 = __uint_as_float(x[c][i]), y1 = __uint_as_float(x[c][i + 1]);
-                            if (MODE == 1 || a.rule.cap > 0.f) {
-                                // 1 - 2/(1 + e), one reciprocal for two elements; at e = 2^60 the tanh is 1 to the last bit
-                                const float e0 = 1.0f + rule_exp2(fminf(y0 * cap_in, 60.f)), e1 = 1.0f + rule_exp2(fminf(y1 * cap_in, 60.f));
-                                const float rr = rule_rcp(e0 * e1) * (-2.0f * cap2);
-                                y0 = fmaf(rr, e1, cap2); y1 = fmaf(rr, e0, cap2);
-                            } else {
-                                y0 *= scale2; y1 *= scale2;
+                        for (uint32_t i = 0; i < 32; i += 2)
+                            top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], fabsf(__uint_as_float(x[c][i])), fabsf(__uint_as_float(x[c][i + 1])));
+                    const bool small = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cap_c <= kTanhSmall;
+                    if (__all_sync(0xffffffffu, small)) {
+#pragma unroll
+                        for (uint32_t c = 0; c < N / 32; ++c)
+#pragma unroll
+                            for (uint32_t i = 0; i < 32; i += 2) cap_small(x[c][i], x[c][i + 1], cap_c, scale2);
+                    } else {
+#pragma unroll
+                        for (uint32_t c = 0; c < N / 32; ++c)
+#pragma unroll
+                            for (uint32_t i = 0; i < 32; i += 2) cap_any(x[c][i], x[c][i + 1], cap_c, cap2);
+                    }
+                }
+                if (MODE == 2) {
+                    const float mul = a.rule.cap > 0.f ? 1.0f : scale2, d0 = (float)(pos - k0);
+                    // rows before the query alone (all but the last tiles, and a prefix behind it): |d| = d
+                    if (__all_sync(0xffffffffu, pos - k0 >= (int32_t)N - 1)) {
+                        const float b0 = -slope2 * d0;
+                        const unsigned long long mul2 = pack_f32x2(mul, mul);
+#pragma unroll
+                        for (uint32_t c = 0; c < N / 32; ++c)
+#pragma unroll
+                            for (uint32_t i = 0; i < 32; i += 2) {
+                                const float col = (float)(c * 32 + i);
+                                float y0, y1;
+                                fma_f32x2(y0, y1, __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]), mul2,
+                                          pack_f32x2(fmaf(slope2, col, b0), fmaf(slope2, col + 1.0f, b0)));
+                                x[c][i] = __float_as_uint(y0); x[c][i + 1] = __float_as_uint(y1);
                             }
-                            if (MODE == 2) {
-                                const float d = (float)(pos - k0 - (int32_t)(c * 32 + i));
-                                y0 = fmaf(-slope2, fabsf(d), y0); y1 = fmaf(-slope2, fabsf(d - 1.0f), y1);
-                            }
-                            x[c][i] = __float_as_uint(y0); x[c][i + 1] = __float_as_uint(y1);
-                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t c = 0; c < N / 32; ++c)
+#pragma unroll
+                            for (uint32_t i = 0; i < 32; ++i)
+                                x[c][i] = __float_as_uint(fmaf(-slope2, fabsf(d0 - (float)(c * 32 + i)), __uint_as_float(x[c][i]) * mul));
+                    }
                 }
                 if (!__all_sync(0xffffffffu, whole)) {
 #pragma unroll
