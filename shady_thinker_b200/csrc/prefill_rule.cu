@@ -16,7 +16,7 @@
 //     One warp finds the items: it walks the sequences' lengths in device memory, latest tokens first, takes every
 //     gridDim.x-th item in serpentine order and works out which K/V tiles a row of it can see (window, documents, prefix),
 //     so nothing is planned on the host and a captured launch serves other lengths.  The other warps take items from a
-//     two-deep ring in shared memory.
+//     ring in shared memory.
 //   * K and V tiles come through rings of their own (a K slot is free once its scores are computed); rows past a
 //     sequence's end may hold anything, so a warp of its own clears them in the V tile (0 * NaN) before the MMA.
 //   * Softmax, one thread per row: the tile's scores are taken to registers whole, transformed, masked by four 32-bit
@@ -51,24 +51,26 @@ template <int HD> struct Cfg {
     static constexpr uint32_t kNT = HD == 128 ? 2 : 1;          // row tiles of an item
     static constexpr uint32_t kN = HD == 128 ? 128 : 64;        // K/V rows of a tile
     static constexpr uint32_t kNS = HD == 128 ? 1 : 3;          // score buffers of a row tile
-    static constexpr uint32_t kAhead = kNS - 1;                 // score tiles issued ahead of the PV of a tile
+    static constexpr uint32_t kAhead = kNS - 1;                 // tiles that the producer fetches K in front of V
     static constexpr uint32_t kSlabs = HD / 64;                 // 64-element (128-byte) slabs of a row
     static constexpr uint32_t kKvSlab = kN * 128, kKvTile = kSlabs * kKvSlab;
     static constexpr uint32_t kQSlab = 128 * 128, kQTile = kSlabs * kQSlab;
     static constexpr uint32_t kKS = 3, kVS = 2;                 // slots of the K and V rings
     static constexpr uint32_t kSmemK = kNT * kQTile, kSmemV = kSmemK + kKS * kKvTile, kSmemMisc = kSmemV + kVS * kKvTile;
-    static constexpr uint32_t kSmem = kSmemMisc + 512 + 1024;   // barriers, item ring; slack for 1024-byte alignment
+    static constexpr uint32_t kSmem = kSmemMisc + 768 + 1024;   // barriers, item ring; slack for 1024-byte alignment
     static constexpr uint32_t kColO = 256;                      // TMEM: scores below, O_q at 256 + 128 q
     static constexpr uint32_t kThreads = kNT * 128 + 128;
     static_assert(kSmem <= 232448, "Q and the rings must fit in 227 KB");
     static_assert(kNT * kNS * kN <= kColO && kColO + kNT * HD <= 512, "TMEM columns");
 };
-enum { B_IFULL = 0, B_IEMPTY = 2, B_QFULL = 4, B_QEMPTY = 6, B_KFULL = 8, B_KEMPTY = 11, B_VFULL = 14, B_VEMPTY = 16, B_VFIX = 18,
-       B_SFULL = 19, B_PFULL = 22, B_OFULL = 25, B_VREQ = 27, B_PVDONE = 28, B_COUNT = 31 };
-constexpr uint32_t kItemOff = 8 * B_COUNT + 16;   // two item descriptors of 16 words behind the barriers, the TMEM slot and the abort word
-static_assert(kItemOff + 2 * 64 <= 512, "barriers and item ring");
+constexpr uint32_t kItems = 4;   // slots of the item ring
+enum { B_IFULL = 0, B_IEMPTY = B_IFULL + kItems, B_QFULL = B_IEMPTY + kItems, B_QEMPTY = B_QFULL + 2, B_KFULL = B_QEMPTY + 2, B_KEMPTY = B_KFULL + 3,
+       B_VFULL = B_KEMPTY + 3, B_VEMPTY = B_VFULL + 2, B_SFULL = B_VEMPTY + 2, B_PFULL = B_SFULL + 3, B_PVDONE = B_PFULL + 3, B_OFULL = B_PVDONE + 3,
+       B_VREQ = B_OFULL + 2, B_VFIX, B_COUNT };
+constexpr uint32_t kItemOff = 8 * B_COUNT + 16;   // item descriptors of 16 words behind the barriers, the TMEM slot and the abort word
+static_assert(kItemOff + kItems * 64 <= 768, "barriers and item ring");
 // The warps of head_dim 128 start with 168 registers each (384 threads); the softmax warpgroups hold a whole row of scores.
-constexpr uint32_t kRegsSoftmax = 216, kRegsOther = 72, kRegsLaunch = 168;
+constexpr uint32_t kRegsSoftmax = 208, kRegsOther = 88, kRegsLaunch = 168;
 static_assert(2 * kRegsSoftmax + kRegsOther <= 3 * kRegsLaunch, "setmaxnreg can only hand out what the block was launched with");
 
 struct Item {
@@ -90,6 +92,12 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
     lo = max(lo, 0); hi = min(hi, 32);
     if (lo >= hi) return 0u;
     return (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
+}
+// whether a phase has completed, without the pause that try_wait may make
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -156,9 +164,11 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const uint32_t TPT = 128u / a.G, R = TPT * a.G, TPI = NT * TPT;   // tokens and rows of a tile, tokens of an item
 
     if (warp == kWProd && lane == 0) {
-        for (uint32_t i = 0; i < 2; ++i) {
+        for (uint32_t i = 0; i < kItems; ++i) {
             mbar_init(bar(B_IFULL + i), 1);
             mbar_init(bar(B_IEMPTY + i), 3 + 4 * NT);   // producer, issuer, V clearing warp, softmax warps
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(bar(B_QFULL + i), 1); mbar_init(bar(B_QEMPTY + i), 1); mbar_init(bar(B_OFULL + i), 1);
         }
         for (uint32_t i = 0; i < C::kKS; ++i) { mbar_init(bar(B_KFULL + i), 1); mbar_init(bar(B_KEMPTY + i), 1); }
@@ -180,10 +190,10 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     // the next item of the ring; false when the list has ended or a wait gave up.  A role of one thread and
     // one of a whole warp differ in who says that the slot has been read.
     auto take_item = [&](uint32_t ic, Item &it, auto whole_warp, int code) {
-        if (!mbar_wait(bar(B_IFULL + (ic & 1)), (ic >> 1) & 1, wc, code)) return false;
-        it = item_read(items + 16 * (ic & 1));
+        if (!mbar_wait(bar(B_IFULL + ic % kItems), (ic / kItems) & 1, wc, code)) return false;
+        it = item_read(items + 16 * (ic % kItems));
         if constexpr (decltype(whole_warp)::value) __syncwarp();
-        if (!decltype(whole_warp)::value || lane == 0) mbar_arrive(bar(B_IEMPTY + (ic & 1)));
+        if (!decltype(whole_warp)::value || lane == 0) mbar_arrive(bar(B_IEMPTY + ic % kItems));
         return it.valid != 0;
     };
     constexpr std::true_type kWarpRole{};
@@ -273,12 +283,12 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                 for (int i = 0; i < 13; ++i) vals[i] = v[i];
             }
-            if (ic >= 2) ok = mbar_wait(bar(B_IEMPTY + (ic & 1)), ((ic >> 1) - 1) & 1, wc, 31);
+            if (ic >= kItems) ok = mbar_wait(bar(B_IEMPTY + ic % kItems), (ic / kItems - 1) & 1, wc, 31);
             if (!ok) break;
             if (lane == 0) {
 #pragma unroll
-                for (int i = 0; i < 13; ++i) items[16 * (ic & 1) + i] = vals[i];
-                mbar_arrive(bar(B_IFULL + (ic & 1)));
+                for (int i = 0; i < 13; ++i) items[16 * (ic % kItems) + i] = vals[i];
+                mbar_arrive(bar(B_IFULL + ic % kItems));
             }
             __syncwarp();
         }
@@ -320,6 +330,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             };
             for (uint32_t ic = 0; ok && take_item(ic, it, kThreadRole, 34); ++ic) {
                 if (!it.n) continue;
+                ok = load_k(0);   // ahead of Q, which waits for the last scores of the item before
                 for (uint32_t q = 0; q < NT && ok; ++q) {
                     if (q * TPT >= it.ntok) continue;
                     if (qn[q] > 0) ok = mbar_wait(bar(B_QEMPTY + q), (qn[q] - 1) & 1, wc, 35);
@@ -332,7 +343,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 }
                 // K runs kAhead + 1 tiles in front of V, as the score MMAs run in front of the PV MMAs
                 for (uint32_t j = 0; j < it.n + C::kAhead && ok; ++j) {
-                    if (j < it.n) ok = load_k(j);
+                    if (j && j < it.n) ok = load_k(j);
                     if (ok && j + 1 > C::kAhead) ok = load_v(j - C::kAhead);
                 }
             }
@@ -375,8 +386,6 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const uint32_t idesc_qk = make_idesc(kFmt, false, N), idesc_pv = make_idesc(kFmt, true, HD);
             bool ok = true;
             uint32_t gk = 0, gv = 0, qn[2] = {0, 0}, sc[2] = {0, 0}, pc[2] = {0, 0}, fixes = 0;
-            Item it{};
-            bool fix = false;
             auto issue_s = [&](uint32_t q, uint32_t b, uint32_t s) {   // scores of row tile q into buffer b from K slot s
                 const uint32_t qa = smem_base + q * C::kQTile, kb = smem_base + C::kSmemK + s * C::kKvTile;
 #pragma unroll
@@ -393,61 +402,86 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     mma_ts(tmem + C::kColO + q * 128, tmem + b * N + ks * 8, desc_mnmajor(vb + ks * 2048, C::kKvSlab), idesc_pv, !first || ks > 0);
             };
             auto wait_k = [&]() { return mbar_wait(bar(B_KFULL + gk % C::kKS), (gk / C::kKS) & 1, wc, 38); };
-            auto wait_v = [&](uint32_t j) {   // tile j of the item has landed, and been cleared past the sequence's end
+            auto wait_v = [&](bool fix) {   // the next V tile has landed, and (the last one of an item that reaches past its sequence) been cleared
                 if (!mbar_wait(bar(B_VFULL + gv % C::kVS), (gv / C::kVS) & 1, wc, 39)) return false;
-                if (!fix || j + 1 != it.n) return true;
+                if (!fix) return true;
                 mbar_arrive(bar(B_VREQ));
                 ++fixes;
                 return mbar_wait(bar(B_VFIX), (fixes - 1) & 1, wc, 40);
             };
-            for (uint32_t ic = 0; ok && take_item(ic, it, kThreadRole, 41); ++ic) {
-                const uint32_t n = it.n;
-                if (!n) continue;
-                fix = (it.tile(n - 1) + 1) * N > it.L;
-                ok = mbar_wait(bar(B_QFULL), qn[0]++ & 1, wc, 42);
-                if (!ok) break;
-                if constexpr (NT == 2) {
-                    // order per K/V tile: S0(j), PV1(j-1), S1(j), PV0(j); the pipe works on one row tile while the other is in its
-                    // softmax.  A commit covers all MMAs issued before it, so S_q(j) complete says PV_q(j-1) complete.
-                    const bool two = it.ntok > TPT;
-                    for (uint32_t j = 0; j <= n && ok; ++j) {
-                        if (j < n) {
-                            if (!(ok = wait_k())) break;
-                            tc_fence_after();
-                            issue_s(0, 0, gk % C::kKS);
-                            if (j == n - 1) tc_commit(bar(B_QEMPTY));
-                            if (!two) { tc_commit(bar(B_KEMPTY + gk % C::kKS)); ++gk; }
-                        }
-                        if (two && j >= 1) {   // V of tile j-1 has been waited for
-                            if (!(ok = mbar_wait(bar(B_PFULL + 1), pc[1]++ & 1, wc, 43))) break;
-                            tc_fence_after();
-                            issue_pv(1, 1, gv % C::kVS, j == 1);
-                            tc_commit(bar(B_VEMPTY + gv % C::kVS));
-                            ++gv;
-                            if (j == n) tc_commit(bar(B_OFULL + 1));
-                        }
-                        if (j < n) {
-                            if (two) {
-                                if (j == 0) {
-                                    if (!(ok = mbar_wait(bar(B_QFULL + 1), qn[1]++ & 1, wc, 44))) break;
-                                    tc_fence_after();
-                                }
-                                issue_s(1, 1, gk % C::kKS);
-                                tc_commit(bar(B_KEMPTY + gk % C::kKS));
-                                ++gk;
-                                if (j == n - 1) tc_commit(bar(B_QEMPTY + 1));
+            uint32_t ic = 0;
+            uint32_t n = 0;             // of the item in hand: K/V tiles; whether its second row tile has tokens; whether its last V
+            bool two = false, fix = false;   // tile reaches past the sequence
+            auto next_item = [&]() {    // the next item with tiles
+                do {
+                    Item i;
+                    if (!take_item(ic++, i, kThreadRole, 41)) return false;
+                    n = i.n;
+                    two = i.ntok > TPT;
+                    fix = n && (i.tile(n - 1) + 1) * N > i.L;
+                } while (!n);
+                return true;
+            };
+            if constexpr (NT == 2) {
+                // order per K/V tile: S0(j), PV1(j-1), S1(j), PV0(j); the pipe works on one row tile while the other is in its
+                // softmax.  A commit covers all MMAs issued before it, so S_q(j) complete says PV_q(j-1) complete.  The stream of
+                // tiles runs on through the items: the first scores of an item are computed while the softmax and the epilogue of
+                // the one before are under way.
+                bool pending = false, p_first = false, p_last = false;   // PV1 of the tile before, of this item or the last one
+                auto pv1 = [&]() {
+                    pending = false;
+                    if (!mbar_wait(bar(B_PFULL + 1), pc[1]++ & 1, wc, 43)) return false;
+                    tc_fence_after();
+                    issue_pv(1, 1, gv % C::kVS, p_first);
+                    tc_commit(bar(B_VEMPTY + gv % C::kVS));
+                    ++gv;
+                    if (p_last) tc_commit(bar(B_OFULL + 1));
+                    return true;
+                };
+                while (ok && next_item()) {
+                    for (uint32_t j = 0; j < n && ok; ++j) {
+                        if (j == 0) {
+                            // across items whichever can go first: the last PV1 of the item before, or the first S0 of this one
+                            auto p1_in = [&]() { return pending && mbar_test(bar(B_PFULL + 1), pc[1] & 1); };
+                            auto s0_in = [&]() { return mbar_test(bar(B_QFULL), qn[0] & 1) && mbar_test(bar(B_KFULL + gk % C::kKS), (gk / C::kKS) & 1); };
+                            for (uint32_t i = 0; pending && i < wc.limit; ++i) {
+                                if (p1_in()) { ok = pv1(); break; }
+                                if (s0_in()) break;
                             }
-                            if (!(ok = wait_v(j))) break;
-                            if (!(ok = mbar_wait(bar(B_PFULL), pc[0]++ & 1, wc, 45))) break;
-                            tc_fence_after();
-                            issue_pv(0, 0, gv % C::kVS, j == 0);
-                            if (!two) { tc_commit(bar(B_VEMPTY + gv % C::kVS)); ++gv; }
-                            if (j == n - 1) tc_commit(bar(B_OFULL));
+                            if (!ok || !(ok = mbar_wait(bar(B_QFULL), qn[0]++ & 1, wc, 42))) break;
                         }
+                        if (!(ok = wait_k())) break;
+                        tc_fence_after();
+                        issue_s(0, 0, gk % C::kKS);
+                        if (j == n - 1) tc_commit(bar(B_QEMPTY));
+                        if (!two) tc_commit(bar(B_KEMPTY + gk % C::kKS));
+                        if (pending && !(ok = pv1())) break;
+                        if (two) {
+                            if (j == 0) {
+                                if (!(ok = mbar_wait(bar(B_QFULL + 1), qn[1]++ & 1, wc, 44))) break;
+                                tc_fence_after();
+                            }
+                            issue_s(1, 1, gk % C::kKS);
+                            tc_commit(bar(B_KEMPTY + gk % C::kKS));
+                            if (j == n - 1) tc_commit(bar(B_QEMPTY + 1));
+                        }
+                        ++gk;
+                        if (!(ok = wait_v(fix && j == n - 1))) break;
+                        if (!(ok = mbar_wait(bar(B_PFULL), pc[0]++ & 1, wc, 45))) break;
+                        tc_fence_after();
+                        issue_pv(0, 0, gv % C::kVS, j == 0);
+                        if (two) { pending = true; p_first = j == 0; p_last = j == n - 1; }
+                        else { tc_commit(bar(B_VEMPTY + gv % C::kVS)); ++gv; }
+                        if (j == n - 1) tc_commit(bar(B_OFULL));
                     }
-                } else {
-                    // one row tile, kAhead score tiles in front of the PV; the buffer of S(j + kAhead) held P(j - 1), whose PV was
-                    // issued before (MMAs of one thread execute in order)
+                }
+                if (ok && pending) pv1();
+            } else {
+                // One row tile, kAhead score tiles in front of the PV; the buffer of S(j + kAhead) held P(j - 1), whose PV was issued
+                // before (MMAs of one thread execute in order).  (Scores that run on into the next item cost this thread more
+                // in polls than they hide: 228 us of the head_dim 256 chunk against 253.)
+                while (ok && next_item()) {
+                    if (!(ok = mbar_wait(bar(B_QFULL), qn[0]++ & 1, wc, 42))) break;
                     auto score = [&](uint32_t j) {
                         if (!wait_k()) return false;
                         tc_fence_after();
@@ -460,14 +494,13 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     for (uint32_t j = 0; j < min(C::kAhead, n) && ok; ++j) ok = score(j);
                     for (uint32_t j = 0; j < n && ok; ++j) {
                         if (j + C::kAhead < n && !(ok = score(j + C::kAhead))) break;
-                        if (!(ok = wait_v(j))) break;
+                        if (!(ok = wait_v(fix && j == n - 1))) break;
                         if (!(ok = mbar_wait(bar(B_PFULL + pc[0] % NS), (pc[0] / NS) & 1, wc, 45))) break;
                         tc_fence_after();
                         issue_pv(0, pc[0] % NS, gv % C::kVS, j == 0);
                         tc_commit(bar(B_VEMPTY + gv % C::kVS));
                         tc_commit(bar(B_PVDONE + pc[0] % NS));
-                        ++pc[0];
-                        ++gv;
+                        ++pc[0]; ++gv;
                         if (j == n - 1) tc_commit(bar(B_OFULL));
                     }
                 }
@@ -485,29 +518,37 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const float cap_c = a.rule.scale * a.rule.inv_cap, cap2 = a.rule.cap * kRuleLog2e;
         bool ok = true;
         uint32_t cnt = 0, oc = 0;   // score tiles and items of this row tile so far (barrier phases)
-        Item it{};
-        for (uint32_t ic = 0; ok && take_item(ic, it, kWarpRole, 46); ++ic) {
-            if (q * TPT >= it.ntok) continue;
-            const bool live = r < R && t_rel < it.ntok;
-            const int32_t pos = it.pos0 + (int32_t)t_rel;
-            const uint32_t head = it.kvh * a.G + g;
+        // (the item's slot is given back behind the epilogue: what a thread does not need between its tiles it reads there again,
+        // instead of holding it beside its row of scores)
+        for (uint32_t ic = 0; ok; ++ic) {
+            if (!(ok = mbar_wait(bar(B_IFULL + ic % kItems), (ic / kItems) & 1, wc, 46))) break;
+            const volatile uint32_t *slot = items + 16 * (ic % kItems);
+            if (!slot[0]) break;
+            auto give_back = [&]() {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_IEMPTY + ic % kItems));
+            };
+            const uint32_t ntok = slot[4], n = slot[11], na = slot[9], b0 = slot[10];
+            if (q * TPT >= ntok) { give_back(); continue; }
+            const bool live = r < R && t_rel < ntok;
+            const int32_t pos = (int32_t)slot[5] + (int32_t)t_rel;
+            int32_t k0 = (int32_t)((na ? slot[8] : b0) * N);   // first row of the tile
             int32_t c_lo = 0, c_hi = 0, p_lo = 0, p_hi = 0;   // rows [c_lo, c_hi) and [p_lo, p_hi) are seen
             if (live && pos >= 0) {
-                p_lo = a.rule.doc ? (int32_t)min(__ldg(a.rule.doc + it.tok0 + t_rel), 0x7fffffffu) : 0;
-                p_hi = (int32_t)it.pre;
+                p_lo = a.rule.doc ? (int32_t)min(__ldg(a.rule.doc + slot[3] + t_rel), 0x7fffffffu) : 0;
+                p_hi = (int32_t)slot[12];
                 c_hi = pos + 1;
                 c_lo = max(p_lo, a.rule.window && (uint32_t)c_hi > a.rule.window ? c_hi - (int32_t)a.rule.window : 0);
             }
             float slope2 = 0.f;
-            if (MODE == 2) slope2 = live ? __ldg(a.rule.slopes + head) * kRuleLog2e : 0.f;
+            if (MODE == 2) slope2 = live ? __ldg(a.rule.slopes + slot[2] * a.G + g) * kRuleLog2e : 0.f;
             float m_ref = -INFINITY, l_sum = 0.f;
-            for (uint32_t j = 0; j < it.n && ok; ++j) {
+            for (uint32_t j = 0; j < n && ok; ++j, k0 = j == na ? (int32_t)(b0 * N) : k0 + (int32_t)N) {
                 const uint32_t b = NT == 2 ? q : cnt % NS;
                 ok = mbar_wait(bar(B_SFULL + b), (NT == 2 ? cnt : cnt / NS) & 1, wc, 47);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t t_s = t_lane + b * N;
-                const int32_t k0 = (int32_t)(it.tile(j) * N);
                 uint32_t x[N / 32][32];
 #pragma unroll
                 for (uint32_t c = 0; c < N / 32; ++c) tmem_ld32(t_s + c * 32, x[c]);
@@ -629,7 +670,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 ++cnt;
             }
             // ---- epilogue: O / l, lse ----
-            if (it.n && ok) {
+            if (n && ok) {
                 ok = mbar_wait(bar(B_OFULL + q), oc & 1, wc, 49);
                 ++oc;
                 if (ok) tc_fence_after();
@@ -637,12 +678,13 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if (!ok) break;
             const bool seen = l_sum > 0.f;
             const float inv = seen ? 1.0f / l_sum : 0.f;
-            const size_t row = ((size_t)it.tok0 + t_rel) * a.nh + head;
+            const size_t row = ((size_t)slot[3] + t_rel) * a.nh + slot[2] * a.G + g;
+            give_back();
             T *dst = reinterpret_cast<T *>(a.out) + row * HD;
 #pragma unroll 2
             for (uint32_t c = 0; c < HD / 32; ++c) {
                 uint32_t v[32];
-                if (it.n) {
+                if (n) {
                     tmem_ld32(t_o + c * 32, v);
                     tmem_wait_ld();
                 }
