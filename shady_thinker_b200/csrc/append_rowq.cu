@@ -209,9 +209,9 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_rowq_kernel(const __
             alignas(8) unsigned char code[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                const int c = rowq_code(x[e], inv);
-                code[e] = (unsigned char)(c + 128);
-                x[e] = (float)c * scale;
+                const float c = rowq_code(x[e], inv);
+                code[e] = (unsigned char)__float_as_uint(c);
+                x[e] = rowq_value(c) * scale;
             }
             if (have_row) {
                 const unsigned long long at = row * a.nkv + kvh;
@@ -256,8 +256,12 @@ int launch_append_rowq(shady_ctx *ctx, const shady_append_params *p, const void 
     a.num_seqs = p->num_seqs; a.tokens_per_seq = p->tokens_per_seq; a.total_tokens = total_tokens;
     a.nh = p->num_heads; a.nkv = p->num_kv_heads; a.has_gate = p->has_gate ? 1u : 0u; a.q_dtype = p->q_dtype;
     a.rd = p->rotary_dim; a.s1 = p->s1_limit; a.s2 = p->s2_limit; a.eps = p->eps;
-    for (uint32_t i = 0; i < p->rotary_dim / 2; ++i)   // the libm call the 16-bit append and the oracle make
-        a.inv_freq[i] = 1.0f / powf(p->rope_theta, 2.0f * (float)i / (float)p->rotary_dim);
+    if (ctx->freq_theta != p->rope_theta || ctx->freq_rd != p->rotary_dim) {   // (64 calls of powf cost a decode step's launch a microsecond)
+        for (uint32_t i = 0; i < p->rotary_dim / 2; ++i)   // the libm call the 16-bit append and the oracle make
+            ctx->freq[i] = 1.0f / powf(p->rope_theta, 2.0f * (float)i / (float)p->rotary_dim);
+        ctx->freq_theta = p->rope_theta; ctx->freq_rd = p->rotary_dim;
+    }
+    for (uint32_t i = 0; i < p->rotary_dim / 2; ++i) a.inv_freq[i] = ctx->freq[i];
     // A warp serves as many vectors of its token as still leave every SM about 48 warps: one each for a decode step,
     // where the launch is latency, the whole token for a prompt, where the angles are then computed once.
     const uint32_t nvec = a.nh + 2 * a.nkv;
@@ -317,41 +321,43 @@ __global__ void __launch_bounds__(kReadThreads) read_rowq_kernel(const __grid_co
         if (lane == 0) sm_row[r] = row;
     }
     __syncthreads();
-    const uint32_t row_pieces = a.nkv * a.hd / 16, head_pieces = a.hd / 16;
-    const uint32_t n = nr * row_pieces;
+    // Eight codes a thread and step: the widest piece whose 16-bit values are one 16-byte store, so that every store
+    // instruction of a warp fills whole sectors.  A thread's row and piece move on by a constant (no division per piece), and
+    // bytes become floats by a byte permute under 2^23 and a subtraction: both kept memory waiting.
+    const uint32_t row_pieces = a.nkv * a.hd / 8, head_shift = 31 - __clz(a.hd / 8);
+    const uint32_t n = nr * row_pieces, step_row = kReadThreads / row_pieces, step_piece = kReadThreads % row_pieces;
     const unsigned char *codes = blockIdx.y ? a.cache.v_codes : a.cache.k_codes;
     const float *scales = blockIdx.y ? a.cache.v_scales : a.cache.k_scales;
     T *out = reinterpret_cast<T *>(blockIdx.y ? a.v_out : a.k_out);
     if (!out) return;
     constexpr uint32_t kUnroll = 4;
+    uint32_t r = tid / row_pieces, piece = tid % row_pieces;
     for (uint32_t i0 = tid; i0 < n; i0 += kReadThreads * kUnroll) {
-        uint4 c[kUnroll];
+        uint2 c[kUnroll];
         float s[kUnroll];
 #pragma unroll
         for (uint32_t u = 0; u < kUnroll; ++u) {
-            const uint32_t i = i0 + u * kReadThreads;
-            c[u] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);   // code 0
+            c[u] = make_uint2(0x80808080u, 0x80808080u);   // code 0
             s[u] = 0.f;
-            if (i < n) {
-                const unsigned long long row = sm_row[i / row_pieces];
-                const uint32_t piece = i % row_pieces;
+            if (i0 + u * kReadThreads < n) {
+                const unsigned long long row = sm_row[r];
                 if (row != ~0ull) {
-                    c[u] = __ldcs(reinterpret_cast<const uint4 *>(codes + row * a.nkv * a.hd) + piece);
-                    s[u] = __ldg(scales + row * a.nkv + piece / head_pieces);
+                    c[u] = __ldcs(reinterpret_cast<const uint2 *>(codes + row * a.nkv * a.hd) + piece);
+                    s[u] = __ldg(scales + row * a.nkv + (piece >> head_shift));
                 }
+                r += step_row; piece += step_piece;
+                if (piece >= row_pieces) { piece -= row_pieces; ++r; }
             }
         }
 #pragma unroll
         for (uint32_t u = 0; u < kUnroll; ++u) {
             const uint32_t i = i0 + u * kReadThreads;
             if (i >= n) break;
-            const unsigned char *b = reinterpret_cast<const unsigned char *>(&c[u]);
-            alignas(16) T v[16];
+            float f[8];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = from_f32<T>((float)((int)b[e] - 128) * s[u]);
-            uint4 *dst = reinterpret_cast<uint4 *>(out + ((size_t)r0 * row_pieces + i) * 16);
-#pragma unroll
-            for (int e = 0; e < (int)sizeof(T); ++e) dst[e] = reinterpret_cast<const uint4 *>(v)[e];
+            for (int e = 0; e < 8; ++e)   // 2^23 + byte, exactly
+                f[e] = (__uint_as_float(__byte_perm(e < 4 ? c[u].x : c[u].y, 0x4b000000u, 0x7540u | (e & 3))) - 8388736.0f) * s[u];
+            vec_store<T, 8>(out + ((size_t)r0 * row_pieces + i) * 8, f);
         }
     }
 }
@@ -371,8 +377,9 @@ int launch_read_rowq(shady_ctx *ctx, const shady_rowq_cache *cache, uint32_t nkv
     if (!total_rows) return SHADY_OK;
     a.row_start = d_row_start; a.out_start = d_out_start; a.k_out = d_k_out; a.v_out = d_v_out;
     a.num_seqs = num_seqs; a.total_rows = total_rows; a.nkv = nkv; a.hd = hd;
-    // rows of a block: about 32 KB of codes of one tensor, fewer while the grid would leave SMs without a block
-    uint32_t rows = 32768u / (nkv * hd);
+    // rows of a block: about 16 KB of codes of one tensor (128k rows of 8 heads of 128: 125 us; 32 KB 130, 64 KB 138), fewer
+    // while the grid would leave SMs without a block
+    uint32_t rows = 16384u / (nkv * hd);
     rows = rows < 1 ? 1 : (rows > kReadMaxRows ? kReadMaxRows : rows);
     while (rows > 1 && (total_rows + rows - 1) / rows < (uint32_t)ctx->num_sms * 4) rows = (rows + 1) / 2;
     a.rows_per_block = rows;

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "../../include/shady_attn.h"
@@ -47,6 +48,10 @@ struct shady_ctx {
     void *stage = nullptr;
     size_t stage_bytes = 0;
     cudaEvent_t stage_done = nullptr;
+    // rotary frequencies of the last (theta, rotary_dim) that the row-scaled append was called with
+    float freq_theta = 0.f;
+    uint32_t freq_rd = ~0u;
+    float freq[128];
 };
 
 // What a kernel needs to report (and notice) an expired wait.
@@ -63,6 +68,15 @@ __device__ __forceinline__ void report_timeout(const StatusRef &st, int code) {
 __device__ __forceinline__ bool gave_up(const StatusRef &st) { return *reinterpret_cast<volatile int *>(st.dev) != 0; }
 
 namespace shady {
+
+// Raises a kernel's dynamic shared memory limit, once per kernel and device (the call costs a launch half a microsecond).
+template <typename K> inline cudaError_t allow_smem_once(K kern, int device, int bytes, std::atomic<uint64_t> &done) {
+    const uint64_t bit = device >= 0 && device < 64 ? 1ull << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // ---- status plumbing ------------------------------------------------------------------
 int fail(shady_ctx *ctx, int code, const std::string &msg);

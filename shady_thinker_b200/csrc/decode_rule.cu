@@ -678,7 +678,8 @@ template <typename T, int HD, bool Q8> static int launch(shady_ctx *ctx, const A
     using S = Smem<HD, Q8>;
     static_assert(S::kCtas <= (int)kMaxCtasPerSm && S::kCtas * (S::kTotal + 1024) <= 228 * 1024, "resident CTAs");
     auto kern = decode_rule_kernel<T, HD, Q8>;
-    SHADY_CUDA_OK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal));
+    static std::atomic<uint64_t> allowed{0};
+    SHADY_CUDA_OK(ctx, allow_smem_once(kern, ctx->device, S::kTotal, allowed));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctx->num_sms * S::kCtas);
     cfg.blockDim = dim3(kThreads);

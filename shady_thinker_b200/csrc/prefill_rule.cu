@@ -740,12 +740,15 @@ struct Maps { CUtensorMap q, k, v; };
 template <typename T, int HD, int MODE> static int launch(shady_ctx *ctx, const Maps &m, const Args &a, uint32_t blocks) {
     using C = Cfg<HD>;
     auto kern = prefill_rule_kernel<T, HD, MODE>;
-    SHADY_CUDA_OK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-    if (C::kNT == 2) {   // a build that launches with fewer registers would wait for them for good
+    static std::atomic<uint64_t> allowed{0};
+    static std::atomic<bool> checked{false};
+    if (C::kNT == 2 && !checked.load(std::memory_order_relaxed)) {   // a build that launches with fewer registers would wait for them for good
         cudaFuncAttributes at{};
         SHADY_CUDA_OK(ctx, cudaFuncGetAttributes(&at, kern));
         SHADY_REQUIRE(ctx, at.numRegs >= (int)kRegsLaunch, SHADY_ERR_UNSUPPORTED, "prefill_rule: this build launches with too few registers per thread");
+        checked.store(true, std::memory_order_relaxed);
     }
+    SHADY_CUDA_OK(ctx, allow_smem_once(kern, ctx->device, C::kSmem, allowed));
     kern<<<blocks, C::kThreads, C::kSmem, ctx->stream>>>(m.q, m.k, m.v, a);
     ctx->launches++;
     SHADY_CUDA_OK(ctx, cudaGetLastError());

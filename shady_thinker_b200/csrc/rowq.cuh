@@ -34,8 +34,15 @@ __device__ __forceinline__ bool rowq_row(const RowqAddr &c, uint32_t s, uint32_t
 
 // scale of a row from its largest magnitude (fmaxf has dropped NaNs on the way; an infinity ends at the upper bound)
 __device__ __forceinline__ float rowq_scale(float amax) { return fminf(fmaxf(amax / kRowqCodeMax, kRowqScaleMin), kRowqScaleMax); }
-// x / scale to the nearest code, -127 .. 127; inv = 1 / scale.  cvt.rni turns a NaN into 0 and saturates infinities.
-__device__ __forceinline__ int rowq_code(float x, float inv) { return max(-127, min(127, __float2int_rn(x * inv))); }
+// x / scale to the nearest code c, -127 .. 127 (a NaN counts as 0), inv = 1 / scale: as the float 1.5 * 2^23 + 128 + c, whose
+// addition rounds to the nearest even integer and whose low byte is the stored code, and c itself from it.  No conversion
+// instruction: those run at an eighth of the rate.
+constexpr float kRowqMagic = 12583040.0f;   // 1.5 * 2^23 + 128
+__device__ __forceinline__ float rowq_code(float x, float inv) {
+    const float v = x * inv;
+    return (v == v ? fminf(fmaxf(v, -127.0f), 127.0f) : 0.0f) + kRowqMagic;
+}
+__device__ __forceinline__ float rowq_value(float code) { return code - kRowqMagic; }
 
 // Checks a caller's description and turns it into the device-side form (append_rowq.cu).
 int fill_rowq_addr(shady_ctx *ctx, const shady_rowq_cache *cache, const char *who, RowqAddr *out);

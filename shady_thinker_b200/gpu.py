@@ -28,16 +28,17 @@ def _addr(buf) -> int:
     """Device address of a Buffer, a torch CUDA tensor, an int, or None."""
     if buf is None:
         return 0
-    if isinstance(buf, Buffer):
-        return buf.ptr
-    if isinstance(buf, int):
-        return buf
-    if hasattr(buf, "data_ptr"):
+    data_ptr = getattr(buf, "data_ptr", None)   # first: most arguments are tensors, and a call has a dozen
+    if data_ptr is not None:
         if not buf.is_cuda:
             raise ValueError("expected a CUDA tensor")
         if not buf.is_contiguous():
             raise ValueError("expected a contiguous tensor")
-        return buf.data_ptr()
+        return data_ptr()
+    if isinstance(buf, Buffer):
+        return buf.ptr
+    if isinstance(buf, int):
+        return buf
     raise TypeError(f"cannot take a device address of {type(buf)}")
 
 
