@@ -17,8 +17,8 @@
 //     gridDim.x-th item in serpentine order and works out which K/V tiles a row of it can see (window, documents, prefix),
 //     so nothing is planned on the host and a captured launch serves other lengths.  The other warps take items from a
 //     ring in shared memory.
-//   * K and V tiles come through rings of their own (a K slot is free once its scores are computed); rows past a
-//     sequence's end may hold anything, so a warp of its own clears them in the V tile (0 * NaN) before the MMA.
+//   * K and V tiles of 64 rows come through rings of their own (a K slot is free once its scores are computed); rows past
+//     a sequence's end may hold anything, so they are cleared in the V tile (0 * NaN) before the MMA.
 //   * Softmax, one thread per row: the tile's scores are taken to registers whole, transformed, masked by four 32-bit
 //     words that interval arithmetic gives (skipped by a warp whose rows see the whole tile), and P goes back over S as
 //     the A operand of the second MMA.  O is only rescaled when a row's maximum grew by more than 2^8.
@@ -49,29 +49,25 @@ struct Args {
 
 template <int HD> struct Cfg {
     static constexpr uint32_t kNT = HD == 128 ? 2 : 1;          // row tiles of an item
-    static constexpr uint32_t kN = HD == 128 ? 128 : 64;        // K/V rows of a tile
-    static constexpr uint32_t kNS = HD == 128 ? 1 : 3;          // score buffers of a row tile
-    static constexpr uint32_t kAhead = kNS - 1;                 // tiles that the producer fetches K in front of V
+    static constexpr uint32_t kN = 64;                          // K/V rows of a tile
+    static constexpr uint32_t kNS = HD == 128 ? 2 : 3;          // score buffers of a row tile: scores are issued that many tiles ahead
     static constexpr uint32_t kSlabs = HD / 64;                 // 64-element (128-byte) slabs of a row
     static constexpr uint32_t kKvSlab = kN * 128, kKvTile = kSlabs * kKvSlab;
     static constexpr uint32_t kQSlab = 128 * 128, kQTile = kSlabs * kQSlab;
-    static constexpr uint32_t kKS = 3, kVS = 2;                 // slots of the K and V rings
+    static constexpr uint32_t kKS = HD == 128 ? 5 : 3, kVS = HD == 128 ? 5 : 2;   // slots of the K and V rings
     static constexpr uint32_t kSmemK = kNT * kQTile, kSmemV = kSmemK + kKS * kKvTile, kSmemMisc = kSmemV + kVS * kKvTile;
     static constexpr uint32_t kSmem = kSmemMisc + 768 + 1024;   // barriers, item ring; slack for 1024-byte alignment
-    static constexpr uint32_t kColO = 256;                      // TMEM: scores below, O_q at 256 + 128 q
+    static constexpr uint32_t kColO = 256;                      // TMEM: scores of row tile q, buffer b at 64 (q kNS + b), O_q at 256 + 128 q
     static constexpr uint32_t kThreads = kNT * 128 + 128;
     static_assert(kSmem <= 232448, "Q and the rings must fit in 227 KB");
     static_assert(kNT * kNS * kN <= kColO && kColO + kNT * HD <= 512, "TMEM columns");
 };
 constexpr uint32_t kItems = 4;   // slots of the item ring
-enum { B_IFULL = 0, B_IEMPTY = B_IFULL + kItems, B_QFULL = B_IEMPTY + kItems, B_QEMPTY = B_QFULL + 2, B_KFULL = B_QEMPTY + 2, B_KEMPTY = B_KFULL + 3,
-       B_VFULL = B_KEMPTY + 3, B_VEMPTY = B_VFULL + 2, B_SFULL = B_VEMPTY + 2, B_PFULL = B_SFULL + 3, B_PVDONE = B_PFULL + 3, B_OFULL = B_PVDONE + 3,
-       B_VREQ = B_OFULL + 2, B_VFIX, B_COUNT };
+enum { B_IFULL = 0, B_IEMPTY = B_IFULL + kItems, B_QFULL = B_IEMPTY + kItems, B_QEMPTY = B_QFULL + 2, B_KFULL = B_QEMPTY + 2, B_KEMPTY = B_KFULL + 5,
+       B_VFULL = B_KEMPTY + 5, B_VEMPTY = B_VFULL + 5, B_SFULL = B_VEMPTY + 5, B_PFULL = B_SFULL + 4, B_PVDONE = B_PFULL + 4, B_OFULL = B_PVDONE + 4,
+       B_COUNT = B_OFULL + 2 };
 constexpr uint32_t kItemOff = 8 * B_COUNT + 16;   // item descriptors of 16 words behind the barriers, the TMEM slot and the abort word
 static_assert(kItemOff + kItems * 64 <= 768, "barriers and item ring");
-// The warps of head_dim 128 start with 168 registers each (384 threads); the softmax warpgroups hold a whole row of scores.
-constexpr uint32_t kRegsSoftmax = 208, kRegsOther = 88, kRegsLaunch = 168;
-static_assert(2 * kRegsSoftmax + kRegsOther <= 3 * kRegsLaunch, "setmaxnreg can only hand out what the block was launched with");
 
 struct Item {
     uint32_t valid, seq, kvh, tok0, ntok;
@@ -79,7 +75,13 @@ struct Item {
     uint32_t L, row0;              // rows of the sequence; its first row in a packed cache
     uint32_t a0, na, b0, n;        // K/V tiles: a0 .. a0+na-1, then b0 ..; n in all
     uint32_t pre;                  // prefix rows
-    __device__ __forceinline__ uint32_t tile(uint32_t j) const { return j < na ? a0 + j : b0 + (j - na); }
+    // Tile j of the item.  With a distance bias the last one comes first: the scores fall from there on, so the running maximum
+    // settles at once (first to last it grew by more than the threshold with every tile, and O was rescaled each time: 231 us
+    // of the head_dim 256 chunk against 165).  Without one the order that ends with the masked tiles is a little faster.
+    template <bool REV> __device__ __forceinline__ uint32_t tile(uint32_t j) const {
+        if (REV) j = n - 1 - j;
+        return j < na ? a0 + j : b0 + (j - na);
+    }
 };
 __device__ __forceinline__ Item item_read(const volatile uint32_t *w) {
     Item it;
@@ -92,12 +94,6 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
     lo = max(lo, 0); hi = min(hi, 32);
     if (lo >= hi) return 0u;
     return (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
-}
-// whether a phase has completed, without the pause that try_wait may make
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -115,19 +111,17 @@ __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigne
     return d;
 }
 __device__ __forceinline__ unsigned long long both(float v) { return pack_f32x2(v, v); }
-// Two raw products s -> cap tanh(s scale / cap) log2(e), with c = scale / cap and scale2 = scale log2(e), for |s c| <=
-// kTanhSmall: a polynomial on the FMA pipe, no special function.  Scores within the cap are the common case: the 4 x 4096
-// batch takes 0.69 ms where exponential and reciprocal per element take 1.06 and a quotient of polynomials for all
-// arguments 1.32.
-__device__ __forceinline__ void cap_small(uint32_t &s0, uint32_t &s1, float c, float scale2) {
-    const unsigned long long s = pack_f32x2(__uint_as_float(s0), __uint_as_float(s1));
-    const unsigned long long x = mul_f32x2(s, both(c)), t = mul_f32x2(x, x);
-    unsigned long long p = fma2(t, both(kTanhC5), both(kTanhC4));
-    p = fma2(p, t, both(kTanhC3));
-    p = fma2(p, t, both(kTanhC2));
-    p = fma2(p, t, both(kTanhC1));
-    p = fma2(p, t, both(kTanhC0));
-    p = mul_f32x2(p, mul_f32x2(s, both(scale2)));   // cap2 x = s scale2
+// Two raw products s -> cap tanh(s scale / cap) log2(e), with c = scale / cap and cap2 = cap log2(e), for |s c| <= kTanhSmall:
+// a polynomial on the FMA pipe, no special function.  Scores within the cap are the common case.  (With an exponential and
+// half a reciprocal per element instead the 4 x 4096 batch took 1.06 ms against 0.90, with a quotient of polynomials for
+// all arguments 1.32.)
+__device__ __forceinline__ void cap_small(uint32_t &s0, uint32_t &s1, float c, float cap2) {
+    const unsigned long long x = mul_f32x2(pack_f32x2(__uint_as_float(s0), __uint_as_float(s1)), both(c)), t = mul_f32x2(x, x);
+    unsigned long long p = fma2(t, both(kTanhC4 * cap2), both(kTanhC3 * cap2));
+    p = fma2(p, t, both(kTanhC2 * cap2));
+    p = fma2(p, t, both(kTanhC1 * cap2));
+    p = fma2(p, t, both(kTanhC0 * cap2));
+    p = mul_f32x2(p, x);
     float y0, y1;
     asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(p));
     s0 = __float_as_uint(y0); s1 = __float_as_uint(y1);
@@ -148,6 +142,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     const __grid_constant__ Args a) {
     using C = Cfg<HD>;
     constexpr uint32_t NT = C::kNT, N = C::kN, NS = C::kNS;
+    constexpr bool kRev = MODE == 2;
     constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;   // swizzled tiles need 1024-byte alignment
@@ -160,21 +155,21 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (gave_up(a.status)) return;
     const WaitCtx wc{abort_word, a.status, a.wait_mbar};
-    constexpr uint32_t kWProd = 4 * NT, kWMma = kWProd + 1, kWSched = kWProd + 2, kWFix = kWProd + 3;
+    constexpr uint32_t kWProd = 4 * NT, kWMma = kWProd + 1, kWSched = kWProd + 2, kWPv = kWProd + 3;
     const uint32_t TPT = 128u / a.G, R = TPT * a.G, TPI = NT * TPT;   // tokens and rows of a tile, tokens of an item
 
     if (warp == kWProd && lane == 0) {
         for (uint32_t i = 0; i < kItems; ++i) {
             mbar_init(bar(B_IFULL + i), 1);
-            mbar_init(bar(B_IEMPTY + i), 3 + 4 * NT);   // producer, issuer, V clearing warp, softmax warps
+            mbar_init(bar(B_IEMPTY + i), 3 + 4 * NT);   // producer, two issuers, softmax warps
         }
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(bar(B_QFULL + i), 1); mbar_init(bar(B_QEMPTY + i), 1); mbar_init(bar(B_OFULL + i), 1);
         }
         for (uint32_t i = 0; i < C::kKS; ++i) { mbar_init(bar(B_KFULL + i), 1); mbar_init(bar(B_KEMPTY + i), 1); }
         for (uint32_t i = 0; i < C::kVS; ++i) { mbar_init(bar(B_VFULL + i), 1); mbar_init(bar(B_VEMPTY + i), 1); }
-        for (uint32_t i = 0; i < 3; ++i) { mbar_init(bar(B_SFULL + i), 1); mbar_init(bar(B_PFULL + i), 128); mbar_init(bar(B_PVDONE + i), 1); }
-        mbar_init(bar(B_VREQ), 1); mbar_init(bar(B_VFIX), 1);
+        for (uint32_t i = 0; i < NT * NS; ++i) { mbar_init(bar(B_SFULL + i), 1); mbar_init(bar(B_PFULL + i), 128); mbar_init(bar(B_PVDONE + i), 1); }
+        
         *abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -200,7 +195,6 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     constexpr std::false_type kThreadRole{};
 
     if (warp >= kWProd) {
-    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == kWSched) {
         // =============================== items ===============================
         // 32 sequences at a time, one per lane.  A sequence's blocks stand at levels [lo, hi) = their first position / TPI; the
@@ -316,7 +310,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const uint32_t s = gk % C::kKS;
                 if (gk >= C::kKS && !mbar_wait(bar(B_KEMPTY + s), (gk / C::kKS - 1) & 1, wc, 32)) return false;
                 mbar_expect_tx(bar(B_KFULL + s), C::kKvTile);
-                load_kv(smem_base + C::kSmemK + s * C::kKvTile, &map_k, bar(B_KFULL + s), it.tile(j) * N);
+                load_kv(smem_base + C::kSmemK + s * C::kKvTile, &map_k, bar(B_KFULL + s), it.template tile<kRev>(j) * N);
                 ++gk;
                 return true;
             };
@@ -324,7 +318,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const uint32_t s = gv % C::kVS;
                 if (gv >= C::kVS && !mbar_wait(bar(B_VEMPTY + s), (gv / C::kVS - 1) & 1, wc, 33)) return false;
                 mbar_expect_tx(bar(B_VFULL + s), C::kKvTile);
-                load_kv(smem_base + C::kSmemV + s * C::kKvTile, &map_v, bar(B_VFULL + s), it.tile(j) * N);
+                load_kv(smem_base + C::kSmemV + s * C::kKvTile, &map_v, bar(B_VFULL + s), it.template tile<kRev>(j) * N);
                 ++gv;
                 return true;
             };
@@ -341,10 +335,10 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     for (uint32_t c = 0; c < C::kSlabs; ++c)
                         tma_load_3d(smem_base + q * C::kQTile + c * C::kQSlab, &map_q, bar(B_QFULL + q), 64 * c, (int)(it.kvh * a.G), (int)(it.tok0 + q * TPT));
                 }
-                // K runs kAhead + 1 tiles in front of V, as the score MMAs run in front of the PV MMAs
-                for (uint32_t j = 0; j < it.n + C::kAhead && ok; ++j) {
-                    if (j && j < it.n) ok = load_k(j);
-                    if (ok && j + 1 > C::kAhead) ok = load_v(j - C::kAhead);
+                // K runs in front of V, as the score MMAs run in front of the PV MMAs
+                for (uint32_t j = 1; j < it.n + NS && ok; ++j) {
+                    if (j < it.n) ok = load_k(j);
+                    if (ok && j >= NS) ok = load_v(j - NS);
                 }
             }
             if (*abort_word || gave_up(a.status)) {   // copies may be in flight: a bounded time for them to land before the memory is handed back
@@ -356,159 +350,82 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     for (uint32_t i = 0; qn[q] && i < (1u << 16) && !mbar_try(bar(B_QFULL + q), (qn[q] - 1) & 1); ++i) {}
             }
         }
-    } else if (warp == kWFix) {
-        // =============================== rows past the sequence's end in its last V tile ===============================
-        // The issuer asks for it once the tile has landed (this warp does not follow the V ring, whose barriers' parity
-        // only tells neighbouring uses of a slot apart).
-        bool ok = true;
-        uint32_t gv = 0, fixes = 0;
-        Item it{};
-        for (uint32_t ic = 0; ok && take_item(ic, it, kWarpRole, 36); ++ic) {
-            if (!it.n) continue;
-            const uint32_t k0 = it.tile(it.n - 1) * N, s = (gv + it.n - 1) % C::kVS;
-            gv += it.n;
-            if (k0 + N <= it.L) continue;
-            ok = mbar_wait(bar(B_VREQ), fixes++ & 1, wc, 37);
-            if (!ok) break;
-            const uint32_t r0 = it.L - k0;   // (the last tile holds a row below L)
-#pragma unroll
-            for (uint32_t c = 0; c < C::kSlabs; ++c) {
-                uint4 *p = reinterpret_cast<uint4 *>(smem + C::kSmemV + s * C::kKvTile + c * C::kKvSlab + r0 * 128);
-                for (uint32_t i = lane; i < (N - r0) * 8; i += 32) p[i] = make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_VFIX));
-        }
-    } else {
-        // =============================== MMA issuer ===============================
+    } else if (warp == kWMma) {
+        // =============================== score MMAs ===============================
+        // Scores and PVs are issued by a thread each: a satisfied wait costs a thread some 250 clocks and a commit 80, and together
+        // they add up to twice what the tensor pipe needs for a tile of 64 rows.  MMAs of different threads are not ordered, so
+        // a score buffer is only overwritten once the PV that read P from it is complete.
         if (lane == 0) {
-            const uint32_t idesc_qk = make_idesc(kFmt, false, N), idesc_pv = make_idesc(kFmt, true, HD);
+            const uint32_t idesc = make_idesc(kFmt, false, N);
             bool ok = true;
-            uint32_t gk = 0, gv = 0, qn[2] = {0, 0}, sc[2] = {0, 0}, pc[2] = {0, 0}, fixes = 0;
-            auto issue_s = [&](uint32_t q, uint32_t b, uint32_t s) {   // scores of row tile q into buffer b from K slot s
-                const uint32_t qa = smem_base + q * C::kQTile, kb = smem_base + C::kSmemK + s * C::kKvTile;
+            uint32_t gk = 0, qn[2] = {0, 0}, qc[2] = {0, 0};   // K and Q tiles, score tiles of each row tile so far
+            Item it{};
+            for (uint32_t ic = 0; ok && take_item(ic, it, kThreadRole, 41); ++ic) {
+                const uint32_t n = it.n, nq = NT == 2 && it.ntok > TPT ? 2u : 1u;
+                for (uint32_t j = 0; j < n && ok; ++j, ++gk) {
+                    for (uint32_t q = 0; q < nq; ++q) {
+                        if (j == 0 && !(ok = mbar_wait(bar(B_QFULL + q), qn[q]++ & 1, wc, 42))) break;
+                        if (q == 0 && !(ok = mbar_wait(bar(B_KFULL + gk % C::kKS), (gk / C::kKS) & 1, wc, 38))) break;
+                        const uint32_t t = qc[q]++, b = q * NS + t % NS;
+                        if (t >= NS && !(ok = mbar_wait(bar(B_PVDONE + b), (t / NS - 1) & 1, wc, 43))) break;
+                        tc_fence_after();
+                        const uint32_t qa = smem_base + q * C::kQTile, kb = smem_base + C::kSmemK + (gk % C::kKS) * C::kKvTile;
 #pragma unroll
-                for (uint32_t ks = 0; ks < HD / 16; ++ks) {
-                    const uint32_t so = ks >> 2, ko = (ks & 3) * 32;
-                    mma_ss(tmem + b * N, desc_kmajor(qa + so * C::kQSlab + ko), desc_kmajor(kb + so * C::kKvSlab + ko), idesc_qk, ks > 0);
+                        for (uint32_t ks = 0; ks < HD / 16; ++ks) {
+                            const uint32_t so = ks >> 2, ko = (ks & 3) * 32;
+                            mma_ss(tmem + b * N, desc_kmajor(qa + so * C::kQSlab + ko), desc_kmajor(kb + so * C::kKvSlab + ko), idesc, ks > 0);
+                        }
+                        tc_commit(bar(B_SFULL + b));
+                        if (q + 1 == nq) tc_commit(bar(B_KEMPTY + gk % C::kKS));
+                        if (j == n - 1) tc_commit(bar(B_QEMPTY + q));
+                    }
                 }
-                tc_commit(bar(B_SFULL + b));
-            };
-            auto issue_pv = [&](uint32_t q, uint32_t b, uint32_t s, bool first) {
-                const uint32_t vb = smem_base + C::kSmemV + s * C::kKvTile;
+            }
+        }
+    } else if (warp == kWPv) {
+        // =============================== PV MMAs ===============================
+        // The whole warp keeps step, because it clears the rows past a sequence's end in its last V tile (0 * NaN) before lane 0
+        // issues the MMA that reads them.
+        const uint32_t idesc = make_idesc(kFmt, true, HD);
+        bool ok = true;
+        uint32_t gv = 0, qc[2] = {0, 0};
+        Item it{};
+        for (uint32_t ic = 0; ok && take_item(ic, it, kWarpRole, 44); ++ic) {
+            const uint32_t n = it.n, nq = NT == 2 && it.ntok > TPT ? 2u : 1u;
+            for (uint32_t j = 0; j < n && ok; ++j, ++gv) {
+                const uint32_t vt = C::kSmemV + (gv % C::kVS) * C::kKvTile;
+                if (!(ok = mbar_wait(bar(B_VFULL + gv % C::kVS), (gv / C::kVS) & 1, wc, 39))) break;
+                const uint32_t k0 = it.template tile<kRev>(j) * N;
+                if (k0 + N > it.L) {
+                    const uint32_t r0 = it.L - k0;   // (an item's last tile holds a row below L)
 #pragma unroll
-                for (uint32_t ks = 0; ks < N / 16; ++ks)
-                    mma_ts(tmem + C::kColO + q * 128, tmem + b * N + ks * 8, desc_mnmajor(vb + ks * 2048, C::kKvSlab), idesc_pv, !first || ks > 0);
-            };
-            auto wait_k = [&]() { return mbar_wait(bar(B_KFULL + gk % C::kKS), (gk / C::kKS) & 1, wc, 38); };
-            auto wait_v = [&](bool fix) {   // the next V tile has landed, and (the last one of an item that reaches past its sequence) been cleared
-                if (!mbar_wait(bar(B_VFULL + gv % C::kVS), (gv / C::kVS) & 1, wc, 39)) return false;
-                if (!fix) return true;
-                mbar_arrive(bar(B_VREQ));
-                ++fixes;
-                return mbar_wait(bar(B_VFIX), (fixes - 1) & 1, wc, 40);
-            };
-            uint32_t ic = 0;
-            uint32_t n = 0;             // of the item in hand: K/V tiles; whether its second row tile has tokens; whether its last V
-            bool two = false, fix = false;   // tile reaches past the sequence
-            auto next_item = [&]() {    // the next item with tiles
-                do {
-                    Item i;
-                    if (!take_item(ic++, i, kThreadRole, 41)) return false;
-                    n = i.n;
-                    two = i.ntok > TPT;
-                    fix = n && (i.tile(n - 1) + 1) * N > i.L;
-                } while (!n);
-                return true;
-            };
-            if constexpr (NT == 2) {
-                // order per K/V tile: S0(j), PV1(j-1), S1(j), PV0(j); the pipe works on one row tile while the other is in its
-                // softmax.  A commit covers all MMAs issued before it, so S_q(j) complete says PV_q(j-1) complete.  The stream of
-                // tiles runs on through the items: the first scores of an item are computed while the softmax and the epilogue of
-                // the one before are under way.
-                bool pending = false, p_first = false, p_last = false;   // PV1 of the tile before, of this item or the last one
-                auto pv1 = [&]() {
-                    pending = false;
-                    if (!mbar_wait(bar(B_PFULL + 1), pc[1]++ & 1, wc, 43)) return false;
+                    for (uint32_t c = 0; c < C::kSlabs; ++c) {
+                        uint4 *p = reinterpret_cast<uint4 *>(smem + vt + c * C::kKvSlab + r0 * 128);
+                        for (uint32_t i = lane; i < (N - r0) * 8; i += 32) p[i] = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                for (uint32_t q = 0; q < nq; ++q) {
+                    const uint32_t t = qc[q]++, b = q * NS + t % NS;
+                    // (a softmax thread reads O of the item before ahead of its arrival here, so the first tile may overwrite it)
+                    if (!(ok = mbar_wait(bar(B_PFULL + b), (t / NS) & 1, wc, 45))) break;
                     tc_fence_after();
-                    issue_pv(1, 1, gv % C::kVS, p_first);
-                    tc_commit(bar(B_VEMPTY + gv % C::kVS));
-                    ++gv;
-                    if (p_last) tc_commit(bar(B_OFULL + 1));
-                    return true;
-                };
-                while (ok && next_item()) {
-                    for (uint32_t j = 0; j < n && ok; ++j) {
-                        if (j == 0) {
-                            // across items whichever can go first: the last PV1 of the item before, or the first S0 of this one
-                            auto p1_in = [&]() { return pending && mbar_test(bar(B_PFULL + 1), pc[1] & 1); };
-                            auto s0_in = [&]() { return mbar_test(bar(B_QFULL), qn[0] & 1) && mbar_test(bar(B_KFULL + gk % C::kKS), (gk / C::kKS) & 1); };
-                            for (uint32_t i = 0; pending && i < wc.limit; ++i) {
-                                if (p1_in()) { ok = pv1(); break; }
-                                if (s0_in()) break;
-                            }
-                            if (!ok || !(ok = mbar_wait(bar(B_QFULL), qn[0]++ & 1, wc, 42))) break;
-                        }
-                        if (!(ok = wait_k())) break;
-                        tc_fence_after();
-                        issue_s(0, 0, gk % C::kKS);
-                        if (j == n - 1) tc_commit(bar(B_QEMPTY));
-                        if (!two) tc_commit(bar(B_KEMPTY + gk % C::kKS));
-                        if (pending && !(ok = pv1())) break;
-                        if (two) {
-                            if (j == 0) {
-                                if (!(ok = mbar_wait(bar(B_QFULL + 1), qn[1]++ & 1, wc, 44))) break;
-                                tc_fence_after();
-                            }
-                            issue_s(1, 1, gk % C::kKS);
-                            tc_commit(bar(B_KEMPTY + gk % C::kKS));
-                            if (j == n - 1) tc_commit(bar(B_QEMPTY + 1));
-                        }
-                        ++gk;
-                        if (!(ok = wait_v(fix && j == n - 1))) break;
-                        if (!(ok = mbar_wait(bar(B_PFULL), pc[0]++ & 1, wc, 45))) break;
-                        tc_fence_after();
-                        issue_pv(0, 0, gv % C::kVS, j == 0);
-                        if (two) { pending = true; p_first = j == 0; p_last = j == n - 1; }
-                        else { tc_commit(bar(B_VEMPTY + gv % C::kVS)); ++gv; }
-                        if (j == n - 1) tc_commit(bar(B_OFULL));
+                    if (lane == 0) {
+#pragma unroll
+                        for (uint32_t ks = 0; ks < N / 16; ++ks)
+                            mma_ts(tmem + C::kColO + q * 128, tmem + b * N + ks * 8, desc_mnmajor(smem_base + vt + ks * 2048, C::kKvSlab), idesc, j > 0 || ks > 0);
+                        tc_commit(bar(B_PVDONE + b));
+                        if (q + 1 == nq) tc_commit(bar(B_VEMPTY + gv % C::kVS));
+                        if (j == n - 1) tc_commit(bar(B_OFULL + q));
                     }
+                    __syncwarp();
                 }
-                if (ok && pending) pv1();
-            } else {
-                // One row tile, kAhead score tiles in front of the PV; the buffer of S(j + kAhead) held P(j - 1), whose PV was issued
-                // before (MMAs of one thread execute in order).  (Scores that run on into the next item cost this thread more
-                // in polls than they hide: 228 us of the head_dim 256 chunk against 253.)
-                while (ok && next_item()) {
-                    if (!(ok = mbar_wait(bar(B_QFULL), qn[0]++ & 1, wc, 42))) break;
-                    auto score = [&](uint32_t j) {
-                        if (!wait_k()) return false;
-                        tc_fence_after();
-                        issue_s(0, sc[0] % NS, gk % C::kKS);
-                        tc_commit(bar(B_KEMPTY + gk % C::kKS));
-                        ++gk; ++sc[0];
-                        if (j == n - 1) tc_commit(bar(B_QEMPTY));
-                        return true;
-                    };
-                    for (uint32_t j = 0; j < min(C::kAhead, n) && ok; ++j) ok = score(j);
-                    for (uint32_t j = 0; j < n && ok; ++j) {
-                        if (j + C::kAhead < n && !(ok = score(j + C::kAhead))) break;
-                        if (!(ok = wait_v(fix && j == n - 1))) break;
-                        if (!(ok = mbar_wait(bar(B_PFULL + pc[0] % NS), (pc[0] / NS) & 1, wc, 45))) break;
-                        tc_fence_after();
-                        issue_pv(0, pc[0] % NS, gv % C::kVS, j == 0);
-                        tc_commit(bar(B_VEMPTY + gv % C::kVS));
-                        tc_commit(bar(B_PVDONE + pc[0] % NS));
-                        ++pc[0]; ++gv;
-                        if (j == n - 1) tc_commit(bar(B_OFULL));
-                    }
-                }
+                ok = __all_sync(0xffffffffu, ok);
             }
         }
     }
     } else {
-        if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         // =============================== softmax (one thread per row) ===============================
         const uint32_t q = warp >> 2, r = tid & 127;
         const uint32_t t_lane = tmem + (((warp & 3) * 32) << 16);
@@ -528,11 +445,13 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(B_IEMPTY + ic % kItems));
             };
-            const uint32_t ntok = slot[4], n = slot[11], na = slot[9], b0 = slot[10];
+            const uint32_t ntok = slot[4], n = slot[11];
             if (q * TPT >= ntok) { give_back(); continue; }
             const bool live = r < R && t_rel < ntok;
             const int32_t pos = (int32_t)slot[5] + (int32_t)t_rel;
-            int32_t k0 = (int32_t)((na ? slot[8] : b0) * N);   // first row of the tile
+            // first row of the tile; the tile at which the order leaves one range for the other, and that one's first tile
+            const uint32_t na = slot[9], turn = kRev ? n - na : na, other = kRev ? slot[8] + na - 1 : slot[10];
+            int32_t k0 = (int32_t)((kRev ? slot[10] + n - na - 1 : (na ? slot[8] : slot[10])) * N);
             int32_t c_lo = 0, c_hi = 0, p_lo = 0, p_hi = 0;   // rows [c_lo, c_hi) and [p_lo, p_hi) are seen
             if (live && pos >= 0) {
                 p_lo = a.rule.doc ? (int32_t)min(__ldg(a.rule.doc + slot[3] + t_rel), 0x7fffffffu) : 0;
@@ -543,9 +462,9 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             float slope2 = 0.f;
             if (MODE == 2) slope2 = live ? __ldg(a.rule.slopes + slot[2] * a.G + g) * kRuleLog2e : 0.f;
             float m_ref = -INFINITY, l_sum = 0.f;
-            for (uint32_t j = 0; j < n && ok; ++j, k0 = j == na ? (int32_t)(b0 * N) : k0 + (int32_t)N) {
-                const uint32_t b = NT == 2 ? q : cnt % NS;
-                ok = mbar_wait(bar(B_SFULL + b), (NT == 2 ? cnt : cnt / NS) & 1, wc, 47);
+            for (uint32_t j = 0; j < n && ok; ++j, k0 = j == turn ? (int32_t)(other * N) : (kRev ? k0 - (int32_t)N : k0 + (int32_t)N)) {
+                const uint32_t b = q * NS + cnt % NS;
+                ok = mbar_wait(bar(B_SFULL + b), (cnt / NS) & 1, wc, 47);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t t_s = t_lane + b * N;
@@ -568,7 +487,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                         for (uint32_t c = 0; c < N / 32; ++c)
 #pragma unroll
-                            for (uint32_t i = 0; i < 32; i += 2) cap_small(x[c][i], x[c][i + 1], cap_c, scale2);
+                            for (uint32_t i = 0; i < 32; i += 2) cap_small(x[c][i], x[c][i + 1], cap_c, cap2);
                     } else {
 #pragma unroll
                         for (uint32_t c = 0; c < N / 32; ++c)
@@ -627,10 +546,10 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     m_ref = mx;
                 }
                 if (__any_sync(0xffffffffu, corr != 1.f)) {
-                    // the PV of the tile before must have written O (its buffer's own barrier: the PVs of up to kAhead tiles may be under way)
-                    if (NT == 1) ok = mbar_wait(bar(B_PVDONE + (cnt - 1) % NS), ((cnt - 1) / NS) & 1, wc, 48);
+                    // the PV of the tile before must have written O (its buffer's own barrier: the PVs of several tiles may be under way)
+                    ok = mbar_wait(bar(B_PVDONE + q * NS + (cnt - 1) % NS), ((cnt - 1) / NS) & 1, wc, 48);
                     if (!ok) break;
-                    if (NT == 1) tc_fence_after();
+                    tc_fence_after();
                     l_sum *= corr;
 #pragma unroll 1
                     for (uint32_t c = 0; c < HD / 16; ++c) {
@@ -741,13 +660,6 @@ template <typename T, int HD, int MODE> static int launch(shady_ctx *ctx, const 
     using C = Cfg<HD>;
     auto kern = prefill_rule_kernel<T, HD, MODE>;
     static std::atomic<uint64_t> allowed{0};
-    static std::atomic<bool> checked{false};
-    if (C::kNT == 2 && !checked.load(std::memory_order_relaxed)) {   // a build that launches with fewer registers would wait for them for good
-        cudaFuncAttributes at{};
-        SHADY_CUDA_OK(ctx, cudaFuncGetAttributes(&at, kern));
-        SHADY_REQUIRE(ctx, at.numRegs >= (int)kRegsLaunch, SHADY_ERR_UNSUPPORTED, "prefill_rule: this build launches with too few registers per thread");
-        checked.store(true, std::memory_order_relaxed);
-    }
     SHADY_CUDA_OK(ctx, allow_smem_once(kern, ctx->device, C::kSmem, allowed));
     kern<<<blocks, C::kThreads, C::kSmem, ctx->stream>>>(m.q, m.k, m.v, a);
     ctx->launches++;

@@ -40,10 +40,9 @@ __device__ __forceinline__ float rule_log2(float x) {
 // which a cap of 50 turns into 2 % of a weight.
 __device__ __forceinline__ float rule_tanh_of_exp(float z2) { return 1.0f - 2.0f * rule_rcp(1.0f + rule_exp2(z2)); }
 
-// tanh(x) = x P(x^2) for |x| <= 1, fitted to the least largest absolute error (Lawson's reweighted least squares): 2.4e-7,
-// in f32 arithmetic 3.2e-7.
-constexpr float kTanhSmall = 1.0f;
-constexpr float kTanhC0 = 0.999996841f, kTanhC1 = -0.333240032f, kTanhC2 = 0.132535249f, kTanhC3 = -0.050972864f, kTanhC4 = 0.0161141828f,
-                kTanhC5 = -0.00283946609f;
+// tanh(x) = x P(x^2) for |x| <= 3/4, fitted to the least largest absolute error (Lawson's reweighted least squares):
+// 1.9e-7, in f32 arithmetic 2.7e-7.
+constexpr float kTanhSmall = 0.75f;
+constexpr float kTanhC0 = 0.999997199f, kTanhC1 = -0.333230764f, kTanhC2 = 0.132260919f, kTanhC3 = -0.0492804497f, kTanhC4 = 0.0123188356f;
 
 }  // namespace shady
