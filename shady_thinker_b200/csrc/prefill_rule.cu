@@ -65,7 +65,7 @@ template <int HD> struct Cfg {
 constexpr uint32_t kItems = 4;   // slots of the item ring
 enum { B_IFULL = 0, B_IEMPTY = B_IFULL + kItems, B_QFULL = B_IEMPTY + kItems, B_QEMPTY = B_QFULL + 2, B_KFULL = B_QEMPTY + 2, B_KEMPTY = B_KFULL + 5,
        B_VFULL = B_KEMPTY + 5, B_VEMPTY = B_VFULL + 5, B_SFULL = B_VEMPTY + 5, B_PFULL = B_SFULL + 4, B_PVDONE = B_PFULL + 4, B_OFULL = B_PVDONE + 4,
-       B_COUNT = B_OFULL + 2 };
+       B_TURN = B_OFULL + 2, B_COUNT = B_TURN + 2 };
 constexpr uint32_t kItemOff = 8 * B_COUNT + 16;   // item descriptors of 16 words behind the barriers, the TMEM slot and the abort word
 static_assert(kItemOff + kItems * 64 <= 768, "barriers and item ring");
 
@@ -165,6 +165,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         for (uint32_t i = 0; i < 2; ++i) {
             mbar_init(bar(B_QFULL + i), 1); mbar_init(bar(B_QEMPTY + i), 1); mbar_init(bar(B_OFULL + i), 1);
+            mbar_init(bar(B_TURN + i), 128);
         }
         for (uint32_t i = 0; i < C::kKS; ++i) { mbar_init(bar(B_KFULL + i), 1); mbar_init(bar(B_KEMPTY + i), 1); }
         for (uint32_t i = 0; i < C::kVS; ++i) { mbar_init(bar(B_VFULL + i), 1); mbar_init(bar(B_VEMPTY + i), 1); }
@@ -434,6 +435,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const float scale2 = a.rule.scale * kRuleLog2e;
         const float cap_c = a.rule.scale * a.rule.inv_cap, cap2 = a.rule.cap * kRuleLog2e;
         bool ok = true;
+        uint32_t tc = 0;            // turns taken
         uint32_t cnt = 0, oc = 0;   // score tiles and items of this row tile so far (barrier phases)
         // (the item's slot is given back behind the epilogue: what a thread does not need between its tiles it reads there again,
         // instead of holding it beside its row of scores)
@@ -561,6 +563,16 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         tmem_st16(t_o + c * 16, v);
                     }
                 }
+                // The two row tiles' scores come together, and both warpgroups would transform them on the FMA pipe and then both
+                // exponentiate on the special function unit.  Taking turns at the exponentials sets them half a tile apart, so
+                // that each pipe is in use throughout.
+                const bool turns = NT == 2 && (MODE == 1 || (MODE == 2 && a.rule.cap > 0.f)) && ntok > TPT;
+                if (turns) {
+                    if (q == 0) ok = tc == 0 || mbar_wait(bar(B_TURN), (tc - 1) & 1, wc, 36);
+                    else ok = mbar_wait(bar(B_TURN + 1), tc & 1, wc, 37);
+                    if (!ok) break;
+                    ++tc;
+                }
                 // ---- P = 2^(x - m), row sum, packed over S ----
                 const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;   // nothing seen yet: every weight is 2^-inf
                 const float mul = MODE == 0 ? scale2 : 1.0f;
@@ -579,6 +591,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     tmem_st16(t_s + c * 16, pk);
                 }
+                if (turns) mbar_arrive(bar(B_TURN + 1 - q));
                 float s0, s1, s2, s3;
                 asm("mov.b64 {%0, %1}, %2;" : "=f"(s0), "=f"(s1) : "l"(ls2[0]));
                 asm("mov.b64 {%0, %1}, %2;" : "=f"(s2), "=f"(s3) : "l"(ls2[1]));
