@@ -462,7 +462,8 @@ typedef struct {
  * (s, j) in row s * tokens_per_seq + j; else device [num_seqs + 1], the first packed token of every sequence (not
  * falling; a sequence may have none), of which total_tokens is an upper bound known to the host: rows of the outputs
  * at or behind d_tok_start[num_seqs] are left as they were.  A position at or behind the end of a sequence's cache
- * (seq_rows, or max_pages_per_seq pages) stores nothing in the cache; its outputs are written all the same. */
+ * (seq_rows, or max_pages_per_seq pages) stores nothing in the cache; its outputs are written all the same.  Two tokens
+ * of a call must not fall on one cache row (pages that two sequences share are read, not appended to). */
 int shady_kv_append_rowq(shady_ctx *ctx, const shady_append_params *p, const void *d_q_proj_full, const void *d_k_proj,
                          const void *d_v_proj, void *d_q_out, float *d_q_gate, void *d_k_out, void *d_v_out,
                          const shady_rowq_cache *cache, const uint16_t *d_qk_norm_bf16, const uint32_t *d_pos_start,
@@ -509,8 +510,10 @@ typedef struct {
  * [num_seqs][nh] f32, natural logarithm of sum exp(z).  Lengths are read on the device only, so a captured launch
  * serves growing sequences.  Rows are cut into equal shares of one resident grid and joined by the CTA that finishes a
  * (sequence, kv head) last, in the order of the shares: results do not depend on which CTA that was.  d_workspace: at
- * least shady_decode_rule_workspace_size bytes, 16-byte aligned, shady_decode_rule_workspace_init once before its
- * first use; every call leaves it ready for the next.  Calls that share a workspace must not overlap on the GPU. */
+ * least shady_decode_rule_workspace_size bytes, 16-byte aligned; shady_decode_rule_workspace_init once before its first
+ * use, with parameters of the largest num_seqs * num_kv_heads (times the groups of eight query heads per kv head) it
+ * will serve, whatever their head_dim.  Every call leaves it ready for the next.  Calls that share a workspace must not
+ * overlap on the GPU. */
 int shady_decode_rule_workspace_size(shady_ctx *ctx, const shady_decode_params *p, size_t *bytes);
 int shady_decode_rule_workspace_init(shady_ctx *ctx, const shady_decode_params *p, void *d_workspace, size_t workspace_bytes);
 int shady_attn_decode_rule(shady_ctx *ctx, const shady_decode_params *p, const shady_score_rule *rule, const void *d_q,

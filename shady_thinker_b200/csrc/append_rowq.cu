@@ -369,6 +369,7 @@ int launch_read_rowq(shady_ctx *ctx, const shady_rowq_cache *cache, uint32_t nkv
     SHADY_REQUIRE(ctx, nkv && num_seqs, SHADY_ERR_BAD_ARG, "kv_read_rowq: zero-sized problem");
     SHADY_REQUIRE(ctx, hd == 64 || hd == 128 || hd == 256, SHADY_ERR_UNSUPPORTED, "kv_read_rowq: head_dim must be 64, 128 or 256");
     SHADY_REQUIRE(ctx, nkv <= 65536, SHADY_ERR_UNSUPPORTED, "kv_read_rowq: too many heads");
+    SHADY_REQUIRE(ctx, total_rows < 0x7fffff00u, SHADY_ERR_UNSUPPORTED, "kv_read_rowq: too many rows for one launch");
     SHADY_REQUIRE(ctx, out_dtype <= SHADY_BF16, SHADY_ERR_BAD_ARG, "kv_read_rowq: bad output dtype");
     SHADY_REQUIRE(ctx, ((uintptr_t)d_k_out & 15) == 0 && ((uintptr_t)d_v_out & 15) == 0, SHADY_ERR_BAD_ARG,
                   "kv_read_rowq: outputs must be 16-byte aligned");

@@ -183,15 +183,15 @@ __device__ __forceinline__ bool visible(const Seq &q, uint32_t row) { return row
 struct OutRef { void *out; float *lse; float *records; uint32_t nh, out_dtype; };
 // four output elements of a head from the weighted sum o and the sum of the weights l
 template <int HD> __device__ __forceinline__ void put_out(const OutRef &a, uint32_t seq, uint32_t head, uint32_t d, const float4 &o, float l) {
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
-    const float v[4] = {l > 0.f ? o.x * inv : 0.f, l > 0.f ? o.y * inv : 0.f, l > 0.f ? o.z * inv : 0.f, l > 0.f ? o.w * inv : 0.f};
+    const float inv = l == 0.f ? 0.f : 1.0f / l;   // nothing seen: zeros (a NaN goes through)
+    const float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
     const size_t at = ((size_t)seq * a.nh + head) * HD + d;
     if (a.out_dtype == SHADY_F32) *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
     else if (a.out_dtype == SHADY_F16) *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(a.out) + at) = make_uint2(pack<__half>(v[0], v[1]), pack<__half>(v[2], v[3]));
     else *reinterpret_cast<uint2 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + at) = make_uint2(pack<__nv_bfloat16>(v[0], v[1]), pack<__nv_bfloat16>(v[2], v[3]));
 }
 __device__ __forceinline__ void put_lse(const OutRef &a, uint32_t seq, uint32_t head, float m, float l) {
-    if (a.lse) a.lse[(size_t)seq * a.nh + head] = l > 0.f ? (m + log2f(l)) * kRuleLn2 : -INFINITY;
+    if (a.lse) a.lse[(size_t)seq * a.nh + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kRuleLn2;
 }
 
 // A CTA joins the records first, first + step, ... (n of them) of a unit into the output, or into record `first`.  Record 0
@@ -203,13 +203,22 @@ __device__ __noinline__ void join(const OutRef a, uint32_t slot0, uint32_t base,
     constexpr int kRec = kHeads * (HD + 2);
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto record = [&](uint32_t k) { return a.records + (size_t)(k ? base + 2 * k : slot0) * kRec; };
+    constexpr uint32_t kUn = 8;   // records requested together
+    auto fetch = [&](float4 (&v)[kUn], uint32_t e, uint32_t k0) {
+        const uint32_t h = e / (HD / 4), d = e % (HD / 4) * 4;
+#pragma unroll
+        for (uint32_t k = 0; k < kUn; ++k)
+            if (k0 + k < n) v[k] = __ldcg(reinterpret_cast<const float4 *>(record(first + (k0 + k) * step) + h * HD + d));
+    };
+    float4 v[kUn];
+    if (tid < heads * (HD / 4)) fetch(v, tid, 0);   // the first ones travel while the factors are worked out
     for (uint32_t h = warp; h < heads; h += kWarps) {   // statistics: a warp per head, its lanes take the records
         float m = -INFINITY, l = 0.f;
         for (uint32_t k = lane; k < n; k += 32) {
-            const float2 v = __ldcg(reinterpret_cast<const float2 *>(record(first + k * step) + kHeads * HD + 2 * h));
-            sm_w[k * kHeads + h] = v.x;
-            const float mn = fmaxf(m, v.x), mu = mn == -INFINITY ? 0.f : mn;
-            l = l * rule_exp2(m - mu) + v.y * rule_exp2(v.x - mu);
+            const float2 st = __ldcg(reinterpret_cast<const float2 *>(record(first + k * step) + kHeads * HD + 2 * h));
+            sm_w[k * kHeads + h] = st.x;
+            const float mn = fmaxf(m, st.x), mu = mn == -INFINITY ? 0.f : mn;
+            l = l * rule_exp2(m - mu) + st.y * rule_exp2(st.x - mu);
             m = mn;
         }
         const float M = warp_max(m), mu = M == -INFINITY ? 0.f : M;
@@ -225,12 +234,8 @@ __device__ __noinline__ void join(const OutRef a, uint32_t slot0, uint32_t base,
     for (uint32_t e = tid; e < heads * (HD / 4); e += kThreads) {
         const uint32_t h = e / (HD / 4), d = e % (HD / 4) * 4;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        constexpr uint32_t kUn = 8;   // records requested together
         for (uint32_t k0 = 0; k0 < n; k0 += kUn) {
-            float4 v[kUn];
-#pragma unroll
-            for (uint32_t k = 0; k < kUn; ++k)
-                if (k0 + k < n) v[k] = __ldcg(reinterpret_cast<const float4 *>(record(first + (k0 + k) * step) + h * HD + d));
+            if (e != tid || k0) fetch(v, e, k0);
 #pragma unroll
             for (uint32_t k = 0; k < kUn; ++k)
                 if (k0 + k < n) {
@@ -623,15 +628,15 @@ __global__ void __launch_bounds__(kThreads, (Smem<HD, Q8>::kCtas)) decode_rule_k
             // share c0 wrote the piece as its last one (slot 1) unless the piece began with the share
             auto slot_of = [&](uint32_t k) { return k ? 2 * (c0 + k) : 2 * c0 + (u0 == c0 * share ? 0u : 1u); };
             auto arrive_last = [&](uint32_t *counter, uint32_t n) {   // all threads: whether this CTA is the n-th; it then leaves the counter at zero
-                __threadfence();
                 __syncthreads();
-                if (tid == 0) *sm_flag = atomicAdd(counter, 1u);
+                if (tid == 0) {   // one thread's fences around the count order what the barriers order for all
+                    __threadfence();
+                    *sm_flag = atomicAdd(counter, 1u);
+                    __threadfence();
+                }
                 __syncthreads();
                 const bool last = *sm_flag == n - 1;
-                if (last) {
-                    __threadfence();
-                    if (tid == 0) *counter = 0;
-                }
+                if (last && tid == 0) *counter = 0;
                 return last;
             };
             float *sm_w = reinterpret_cast<float *>(sm_ring);
@@ -661,18 +666,22 @@ static int check(shady_ctx *ctx, const shady_decode_params *p) {
                   SHADY_ERR_BAD_ARG, "decode_rule: num_q_heads must be num_kv_heads * heads_per_kv");
     SHADY_REQUIRE(ctx, p->head_dim == 64 || p->head_dim == 128 || p->head_dim == 256, SHADY_ERR_UNSUPPORTED,
                   "decode_rule: head_dim must be 64, 128 or 256");
+    SHADY_REQUIRE(ctx, (unsigned long long)p->num_seqs * p->num_kv_heads * head_groups(p) <= 0x4000000ull, SHADY_ERR_UNSUPPORTED,
+                  "decode_rule: too many sequences and heads for one launch");
+    SHADY_REQUIRE(ctx, (unsigned long long)p->num_kv_heads * p->head_dim <= 0x10000000ull, SHADY_ERR_UNSUPPORTED, "decode_rule: too many kv heads");
     SHADY_REQUIRE(ctx, p->num_splits == 0, SHADY_ERR_UNSUPPORTED, "decode_rule: num_splits must be 0 (shares are worked out on the device)");
     SHADY_REQUIRE(ctx, p->q_dtype <= SHADY_BF16 && p->out_dtype <= SHADY_BF16, SHADY_ERR_BAD_ARG, "decode_rule: bad dtype");
     return SHADY_OK;
 }
 constexpr uint32_t kMaxCtasPerSm = 3;
+// Workspace: the records of the widest head_dim, then the counters.  The counters thus lie in the same place for every shape,
+// and one workspace serves several.
+static size_t record_bytes(const shady_ctx *ctx) { return (size_t)2 * ctx->num_sms * kMaxCtasPerSm * kHeads * (256 + 2) * 4; }
 static size_t group_words(const shady_ctx *ctx) { return (size_t)2 * ctx->num_sms * kMaxCtasPerSm; }
 static size_t counter_bytes(const shady_ctx *ctx, const shady_decode_params *p) {
     return (((size_t)p->num_seqs * p->num_kv_heads * head_groups(p) + group_words(ctx)) * 4 + 255) & ~(size_t)255;
 }
-static size_t workspace_bytes(const shady_ctx *ctx, const shady_decode_params *p) {
-    return counter_bytes(ctx, p) + (size_t)2 * ctx->num_sms * kMaxCtasPerSm * kHeads * (p->head_dim + 2) * 4;
-}
+static size_t workspace_bytes(const shady_ctx *ctx, const shady_decode_params *p) { return record_bytes(ctx) + counter_bytes(ctx, p); }
 
 template <typename T, int HD, bool Q8> static int launch(shady_ctx *ctx, const Args &a) {
     using S = Smem<HD, Q8>;
@@ -706,8 +715,9 @@ int decode_rule_workspace_size(shady_ctx *ctx, const shady_decode_params *p, siz
 }
 int decode_rule_workspace_init(shady_ctx *ctx, const shady_decode_params *p, void *d_ws, size_t ws_bytes) {
     if (const int st = dr::check(ctx, p)) return st;
-    SHADY_REQUIRE(ctx, d_ws && ws_bytes >= dr::workspace_bytes(ctx, p), SHADY_ERR_WORKSPACE, "decode_rule: workspace missing or too small");
-    SHADY_CUDA_OK(ctx, cudaMemsetAsync(d_ws, 0, dr::counter_bytes(ctx, p), ctx->stream));
+    SHADY_REQUIRE(ctx, d_ws && ((uintptr_t)d_ws & 15) == 0 && ws_bytes >= dr::workspace_bytes(ctx, p), SHADY_ERR_WORKSPACE,
+                  "decode_rule: workspace missing, unaligned or too small");
+    SHADY_CUDA_OK(ctx, cudaMemsetAsync(reinterpret_cast<char *>(d_ws) + dr::record_bytes(ctx), 0, dr::counter_bytes(ctx, p), ctx->stream));
     return SHADY_OK;
 }
 
@@ -732,9 +742,9 @@ int launch_decode_rule(shady_ctx *ctx, const shady_decode_params *p, const shady
     SHADY_REQUIRE(ctx, d_ws && ((uintptr_t)d_ws & 15) == 0 && ws_bytes >= dr::workspace_bytes(ctx, p), SHADY_ERR_WORKSPACE,
                   "decode_rule: workspace missing, unaligned or too small");
     a.q = d_q; a.out = d_out; a.lse = d_lse; a.lens = d_seq_lens;
-    a.group_counters = reinterpret_cast<uint32_t *>(d_ws);
+    a.records = reinterpret_cast<float *>(d_ws);
+    a.group_counters = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(d_ws) + dr::record_bytes(ctx));
     a.counters = a.group_counters + dr::group_words(ctx);
-    a.records = reinterpret_cast<float *>(reinterpret_cast<char *>(d_ws) + dr::counter_bytes(ctx, p));
     a.num_seqs = p->num_seqs; a.nkv = p->num_kv_heads; a.nh = p->num_q_heads; a.G = a.nh / a.nkv; a.groups = dr::head_groups(p);
     a.q_dtype = p->q_dtype; a.out_dtype = p->out_dtype;
     a.pad = dr::kPad;

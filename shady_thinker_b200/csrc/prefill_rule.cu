@@ -131,8 +131,10 @@ __device__ __forceinline__ void cap_small(uint32_t &s0, uint32_t &s1, float c, f
 __device__ __forceinline__ void cap_any(uint32_t &s0, uint32_t &s1, float c, float cap2) {
     const float ci = c * (2.0f * kRuleLog2e);
     const float e0 = 1.0f + rule_exp2(fminf(__uint_as_float(s0) * ci, 60.f)), e1 = 1.0f + rule_exp2(fminf(__uint_as_float(s1) * ci, 60.f));
-    const float r = rule_rcp(e0 * e1) * (-2.0f * cap2);
-    s0 = __float_as_uint(fmaf(r, e1, cap2)); s1 = __float_as_uint(fmaf(r, e0, cap2));
+    const float r = rule_rcp(e0 * e1) * (-2.0f * cap2), y0 = fmaf(r, e1, cap2), y1 = fmaf(r, e0, cap2);
+    // (fminf has kept a NaN of one element out of the other, whose row may be the sequence's last)
+    if (__uint_as_float(s0) == __uint_as_float(s0)) s0 = __float_as_uint(y0);
+    if (__uint_as_float(s1) == __uint_as_float(s1)) s1 = __float_as_uint(y1);
 }
 
 // MODE 0: scale only, 1: tanh cap, 2: distance bias, with or without a cap
@@ -608,7 +610,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (ok) tc_fence_after();
             }
             if (!ok) break;
-            const bool seen = l_sum > 0.f;
+            const bool seen = l_sum != 0.f;   // (a NaN goes through)
             const float inv = seen ? 1.0f / l_sum : 0.f;
             const size_t row = ((size_t)slot[3] + t_rel) * a.nh + slot[2] * a.G + g;
             give_back();
@@ -700,6 +702,7 @@ int launch_prefill_rule(shady_ctx *ctx, const shady_prefill_params *p, const sha
     SHADY_REQUIRE(ctx, p->dtype == SHADY_F16 || p->dtype == SHADY_BF16, SHADY_ERR_UNSUPPORTED, w + ": dtype must be f16 or bf16");
     SHADY_REQUIRE(ctx, cache->dtype == p->dtype, SHADY_ERR_UNSUPPORTED, w + ": the cache must have the dtype of Q");
     SHADY_REQUIRE(ctx, !cache->d_k_ptrs && !cache->d_v_ptrs, SHADY_ERR_UNSUPPORTED, w + ": pointer-array caches are not supported");
+    SHADY_REQUIRE(ctx, total_q < 0x7fffff00u, SHADY_ERR_UNSUPPORTED, w + ": too many tokens");
     SHADY_REQUIRE(ctx, cache_rows < 0x7fffff00ull, SHADY_ERR_UNSUPPORTED, w + ": too many cache rows");
     for (const void *ptr : {d_q, (const void *)d_out, (const void *)cache->d_k_base, (const void *)cache->d_v_base})
         SHADY_REQUIRE(ctx, ((uintptr_t)ptr & 15) == 0, SHADY_ERR_BAD_ARG, w + ": tensors must be 16-byte aligned");

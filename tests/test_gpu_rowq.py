@@ -137,8 +137,8 @@ def test_append_matches_the_definition(gpu_ctx, hd, nkv, G, dt, q_dt, gate, rd, 
         assert t_ is None or bool((t_[n:] == 7.0).all())                        # rows behind the last token
 
 
-def test_append_uniform_equals_packed_and_replays(gpu_ctx):
-    """The uniform call, the packed call with equal counts, and two replays of a captured launch write the same bytes."""
+def test_append_uniform_equals_packed(gpu_ctx):
+    """The uniform call and the packed call with equal counts write the same bytes."""
     g = torch.Generator().manual_seed(4)
     S, T, nkv, G, hd = 3, 5, 2, 4, 128
     n, nh = S * T, nkv * G
@@ -152,6 +152,50 @@ def test_append_uniform_equals_packed_and_replays(gpu_ctx):
         assert torch.equal(x, y)
     for i in range(2):
         assert torch.equal(a.codes[i], b.codes[i])
+
+
+def test_append_and_read_captured(gpu_ctx):
+    """Append and read-back captured together and replayed with other positions, counts and rows in the same device buffers."""
+    from shady_thinker_b200.gpu import GpuContext
+    S, nkv, G, hd, most = 3, 2, 2, 64, 12
+    stream = torch.cuda.Stream()
+    gpu = GpuContext(0, stream=stream.cuda_stream)
+    c = Cache([50] * S, nkv, hd, 16)
+    g = torch.Generator().manual_seed(7)
+    k, v = (torch.randn(most, nkv, hd, generator=g) for _ in range(2))
+    with torch.cuda.stream(stream):
+        kd, vd, q = k.cuda(), v.cuda(), torch.randn(most, nkv * G, hd, generator=g).cuda()
+        qo, ko, vo = torch.zeros_like(q), torch.zeros_like(kd), torch.zeros_like(vd)
+        kr, vr = torch.zeros_like(kd), torch.zeros_like(vd)
+        pos, starts = dev_u32([0, 0, 0]), dev_u32([0, 1, 2, 3])
+
+        def call():
+            ops.kv_append_rowq(gpu, q_proj_full=q, k_proj=kd, v_proj=vd, q_out=qo, q_gate=None, k_out=ko, v_out=vo, cache=c.view, pos_start=pos,
+                               num_heads=nkv * G, num_kv_heads=nkv, head_dim=hd, rope_theta=1e4, rotary_dim=0, num_seqs=S, tokens_per_seq=0,
+                               tok_start=starts, total_tokens=most, has_gate=False)
+            ops.kv_read_rowq(gpu, cache=c.view, k_out=kr, v_out=vr, row_start=pos, out_start=starts, total_rows=most, num_seqs=S,
+                             num_kv_heads=nkv, head_dim=hd, out_dtype=F32)
+        call()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call()
+        for p, counts in (([5, 49, 17], [3, 1, 8]), ([40, 0, 3], [0, 9, 1])):
+            pos.copy_(dev_u32(p))
+            starts.copy_(dev_u32([0] + list(np.cumsum(counts))))
+            for t in (ko, vo, kr, vr):
+                t.fill_(7.0)
+            graph.replay()
+            stream.synchronize()
+            n = sum(counts)
+            for x, out, back in ((k, ko, kr), (v, vo, vr)):
+                code, scale = quantise(x[:n])
+                held = (code.float() - 128) * scale[..., None]
+                assert torch.equal(back, out) and bool((out[n:] == 7.0).all())
+                assert float((out[:n].cpu() - held).abs().max()) <= float(scale.max()) * (1 + 2.0 ** -12)   # a code at most one apart
+    gpu.synchronize()
+    del graph
+    gpu.close()
 
 
 def test_mrope_sections_match_the_16_bit_append(gpu_ctx):

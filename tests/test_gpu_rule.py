@@ -439,3 +439,164 @@ def test_refusals(gpu_ctx):
     with pytest.raises(ShadyError):
         ops.decode_rule_workspace_size(gpu_ctx, head_dim=100, num_kv_heads=nkv, num_q_heads=nh, num_seqs=S)
     assert cq.view.seq_rows == 20
+
+
+# ---- calls that the documentation allows and a careless kernel gets wrong --------------------------------------------
+
+def test_decode_workspace_serves_several_shapes(gpu_ctx):
+    """One workspace, initialised for the largest batch, used by calls of other head_dims, groups and cache kinds in turn."""
+    ws = workspace(gpu_ctx, 64, 3, 48, 40)                    # 40 sequences, 3 kv heads of two head groups
+    for hd, nkv, G, lens in ((128, 2, 4, [700, 3]), (64, 3, 16, [90] * 40), (256, 1, 8, [3000]), (128, 2, 4, [900, 44, 0, 17])):
+        c = Rows16(lens, nkv, hd, F16, "stride")
+        check_decode(gpu_ctx, c, c.values, lens, nkv, G, hd, F16, F16, torch.float16, dict(cap=20.0), ws=ws)
+        cq = RowsQ(lens, nkv, hd, 16, seed=hd)
+        held = cq.held()
+        check_decode(gpu_ctx, cq, lambda s: held[s], lens, nkv, G, hd, F16, F32, torch.float16, {}, ws=ws)
+
+
+def test_decode_two_calls_at_once(gpu_ctx):
+    """Two contexts on two streams, a workspace each, many launches in flight together."""
+    from shady_thinker_b200.gpu import GpuContext
+    nkv, G, hd, lens = 2, 4, 128, [600, 41]
+    c = Rows16(lens, nkv, hd, F16, "stride")
+    g = torch.Generator().manual_seed(1)
+    q = [(2 * torch.randn(2, nkv * G, hd, generator=g)).half().cuda() for _ in range(2)]
+    ld = dev_u32(lens)
+    want = []
+    for i in range(2):
+        ws, n = workspace(gpu_ctx, hd, nkv, nkv * G, 2)
+        o = torch.empty_like(q[i])
+        ops.attn_decode_rule(gpu_ctx, q=q[i], cache=c.view, seq_lens=ld, out=o, head_dim=hd, num_kv_heads=nkv, num_q_heads=nkv * G, num_seqs=2,
+                             q_dtype=F16, out_dtype=F16, workspace=ws, workspace_bytes=n)
+        want.append(o)
+    gpu_ctx.synchronize()
+    ctx = [GpuContext(0) for _ in range(2)]
+    wss = [workspace(x, hd, nkv, nkv * G, 2) for x in ctx]
+    outs = [[torch.empty_like(q[0]) for _ in range(30)] for _ in range(2)]
+    for x in ctx:
+        x.synchronize()
+    torch.cuda.synchronize()
+    for k in range(30):
+        for i in range(2):
+            ops.attn_decode_rule(ctx[i], q=q[i], cache=c.view, seq_lens=ld, out=outs[i][k], head_dim=hd, num_kv_heads=nkv, num_q_heads=nkv * G,
+                                 num_seqs=2, q_dtype=F16, out_dtype=F16, workspace=wss[i][0], workspace_bytes=wss[i][1])
+    for x in ctx:
+        x.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
+    for x in ctx:
+        x.close()
+
+
+def test_decode_length_behind_the_cache_reads_no_other_sequence(gpu_ctx):
+    """A length larger than a row-scaled sequence's cache: rows that it does not have count as zero rows, none of the next
+    sequence's (here NaN) is read."""
+    c = RowsQ([40, 40], 1, 64, seed=1)
+    c.scales[0][40:] = float("nan")
+    q = torch.randn(1, 4, 64, generator=torch.Generator().manual_seed(1)).half().cuda()
+    out = torch.empty_like(q)
+    ws, n = workspace(gpu_ctx, 64, 1, 4, 1)
+    ops.attn_decode_rule(gpu_ctx, q=q, cache=c.view, seq_lens=dev_u32([70]), out=out, head_dim=64, num_kv_heads=1, num_q_heads=4, num_seqs=1,
+                         q_dtype=F16, out_dtype=F16, workspace=ws, workspace_bytes=n)
+    gpu_ctx.synchronize()
+    assert bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("cap", [0.0, 3.0])
+def test_nan_queries_give_nan_and_stay_in_their_row(gpu_ctx, cap):
+    nkv, G, hd, L = 1, 4, 128, 200
+    c = Rows16([L], nkv, hd, BF16, "stride")
+    cq = RowsQ([L], nkv, hd, seed=2)
+    rule = ops.ScoreRule(cap=cap)
+    q = torch.randn(1, G, hd, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    q[0, 2, 5] = float("nan")
+    ws, n = workspace(gpu_ctx, hd, nkv, G, 1)
+    for cache, kw in ((c.view, {}), (cq.view, {})):
+        out, lse = torch.zeros(1, G, hd, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, G, device="cuda")
+        ops.attn_decode_rule(gpu_ctx, q=q.cuda(), cache=cache, seq_lens=dev_u32([L]), out=out, lse=lse, rule=rule, head_dim=hd, num_kv_heads=nkv,
+                             num_q_heads=G, num_seqs=1, q_dtype=BF16, out_dtype=BF16, workspace=ws, workspace_bytes=n)
+        gpu_ctx.synchronize()
+        assert bool(out[0, 2].isnan().all()) and bool(lse[0, 2].isnan())
+        assert bool(out[0, [0, 1, 3]].isfinite().all()) and bool(lse[0, [0, 1, 3]].isfinite().all())
+    qp = torch.randn(L, G, hd, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    qp[100, 1, 7] = float("nan")
+    out, lse = torch.zeros(L, G, hd, dtype=torch.bfloat16, device="cuda"), torch.zeros(L, G, device="cuda")
+    ops.attn_prefill_rule(gpu_ctx, q=qp.cuda(), cache=c.view, cache_rows=c.rows, q_starts=dev_u32([0, L]), kv_lens=dev_u32([L]), out=out, lse=lse,
+                          rule=rule, head_dim=hd, num_kv_heads=nkv, num_q_heads=G, num_seqs=1, total_q=L, dtype=BF16)
+    gpu_ctx.synchronize()
+    bad = torch.zeros(L, G, dtype=torch.bool)
+    bad[100, 1] = True
+    assert torch.equal(out.isnan().all(-1).cpu(), bad) and torch.equal(out.isnan().any(-1).cpu(), bad) and torch.equal(lse.isnan().cpu(), bad)
+
+
+@pytest.mark.parametrize("scale,cap", [(1.0, 1e6), (1e-3, 1e6), (5.0, 1.0), (1.0, 0.01), (0.088, 2.0)])
+def test_caps_far_from_the_scores(gpu_ctx, scale, cap):
+    """Caps that no score comes near (the polynomial's coefficients would leave f32's range), and that every score exceeds."""
+    rule = dict(scale=scale, cap=cap)
+    lens = [150]
+    c = Rows16(lens, 1, 128, BF16, "packed")
+    check_prefill(gpu_ctx, c, c.values, [150], lens, 1, 2, 128, BF16, rule)
+    d = Rows16(lens, 1, 128, BF16, "stride")
+    check_decode(gpu_ctx, d, d.values, lens, 1, 2, 128, BF16, BF16, torch.bfloat16, rule)
+
+
+def test_prefill_captured_launch_serves_other_lengths(gpu_ctx):
+    """One captured launch, replayed with other token counts and lengths in the same device buffers, padded behind."""
+    from shady_thinker_b200.gpu import GpuContext
+    nkv, G, hd, S, most = 1, 2, 128, 3, 260
+    nh = nkv * G
+    stream = torch.cuda.Stream()
+    gpu = GpuContext(0, stream=stream.cuda_stream)
+    c = Rows16([300, 300, 300], nkv, hd, F16, "stride")
+    q = (2 * torch.randn(most, nh, hd, generator=torch.Generator().manual_seed(3))).half()
+    with torch.cuda.stream(stream):
+        qd, starts, lens = q.cuda(), dev_u32([0, 1, 2, 3]), dev_u32([1, 1, 1])
+        out = torch.zeros(most, nh, hd, dtype=torch.float16, device="cuda")
+        call = lambda: ops.attn_prefill_rule(gpu, q=qd, cache=c.view, cache_rows=c.rows, q_starts=starts, kv_lens=lens, out=out, head_dim=hd,  # noqa: E731
+                                             num_kv_heads=nkv, num_q_heads=nh, num_seqs=S, total_q=most, dtype=F16)
+        call()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call()
+        for counts, rows in (([100, 0, 160], [300, 7, 200]), ([1, 130, 5], [1, 130, 299])):
+            at = [0] + [int(x) for x in np.cumsum(counts)]
+            starts.copy_(dev_u32(at))
+            lens.copy_(dev_u32(rows))
+            out.fill_(7.0)
+            graph.replay()
+            stream.synchronize()
+            assert bool((out[at[-1]:] == 7.0).all())
+            for s in range(S):
+                k, v = (x[:rows[s]] for x in c.values(s))
+                for i in {0, counts[s] // 2, counts[s] - 1} if counts[s] else ():
+                    want, _, b, _ = attend(q[at[s] + i, 1].double(), k[:, 0], v[:, 0], rows[s] - counts[s] + i, rows[s], wt=torch.float16, out_dt=torch.float16)
+                    assert bool(((out[at[s] + i, 1].cpu().double() - want).abs() <= b).all()), (s, i)
+    gpu.synchronize()
+    del graph
+    gpu.close()
+
+
+def test_prefill_pages_that_the_pool_does_not_have(gpu_ctx):
+    """Table entries behind the pool read as zero rows instead of faulting."""
+    L, pr = 100, 16
+    c = Rows16([L], 1, 128, F16, "paged", page_rows=pr)
+    table = c.keep[2].clone()
+    table[0, 2], table[0, 4] = 0x7ffffff0, -1                # rows 32..47 and 64..79
+    c.view.page_table = table
+    c.kv[0][0], c.kv[1][0] = c.kv[0][0].clone(), c.kv[1][0].clone()
+    for t in (c.kv[0][0], c.kv[1][0]):
+        t[32:48] = 0
+        t[64:80] = 0
+    check_prefill(gpu_ctx, c, c.values, [L], [L], 1, 2, 128, F16, {})
+
+
+def test_prefill_many_short_sequences_and_gaps(gpu_ctx):
+    """More sequences than a warp has lanes, some without tokens, contexts of very different lengths (levels with gaps)."""
+    g = torch.Generator().manual_seed(3)
+    kv_lens = [int(x) for x in torch.randint(1, 60, (70,), generator=g)]
+    kv_lens[5], kv_lens[40] = 3000, 900
+    q_lens = [min(L, int(x)) for L, x in zip(kv_lens, torch.randint(0, 9, (70,), generator=g))]
+    q_lens[5], q_lens[40], q_lens[69] = 3, 700, 0
+    c = Rows16(kv_lens, 1, 128, BF16, "packed")
+    check_prefill(gpu_ctx, c, c.values, q_lens, kv_lens, 1, 4, 128, BF16, dict(cap=25.0), heads=[0, 3])
