@@ -184,9 +184,18 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         for (uint32_t i = 0; i < C::kKS; ++i) { mbar_init(bar(B_KFULL + i), 1); mbar_init(bar(B_KEMPTY + i), 1); }
         for (uint32_t i = 0; i < C::kVS; ++i) { mbar_init(bar(B_VFULL + i), 1); mbar_init(bar(B_VEMPTY + i), 1); }
         for (uint32_t i = 0; i < NT * NS; ++i) { mbar_init(bar(B_SFULL + i), 1); mbar_init(bar(B_PFULL + i), 128); mbar_init(bar(B_PVDONE + i), 1); }
-        
         *abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // Where G does not divide 128 the Q boxes leave the last rows of a tile alone.  Nobody reads their results, but their scores
+    // go through the same warps, and what shared memory happened to hold sent a whole warp down the wide branch of the cap
+    // (2 x 2155 tokens, 6 heads per kv head, cap 50: 155 us; with the rows cleared 101).
+    if (R < 128) {
+        for (uint32_t c = 0; c < NT * C::kSlabs; ++c) {
+            uint4 *p = reinterpret_cast<uint4 *>(smem + (c / C::kSlabs) * C::kQTile + (c % C::kSlabs) * C::kQSlab + R * 128u);
+            for (uint32_t i = tid; i < (128u - R) * 8; i += C::kThreads) p[i] = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == kWMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_slot)), "r"(512u) : "memory");
