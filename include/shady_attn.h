@@ -509,7 +509,9 @@ typedef struct {
  * cache after a power of two per head has been taken out); p->out_dtype any of the three.  d_lse: optional
  * [num_seqs][nh] f32, natural logarithm of sum exp(z).  Lengths are read on the device only, so a captured launch
  * serves growing sequences.  Rows are cut into equal shares of one resident grid and joined by the CTA that finishes a
- * (sequence, kv head) last, in the order of the shares: results do not depend on which CTA that was.  d_workspace: at
+ * (sequence, kv head) last, in the order of the shares: results do not depend on which CTA that was.  The V scales of the
+ * rows that a query of a row-scaled cache sees may lie up to 2^100 apart: a row whose scale is further below the largest
+ * one's than that may be missing from the sum of the weights.  d_workspace: at
  * least shady_decode_rule_workspace_size bytes, 16-byte aligned; shady_decode_rule_workspace_init once before its first
  * use, with parameters of the largest num_seqs * num_kv_heads (times the groups of eight query heads per kv head) it
  * will serve, whatever their head_dim.  Every call leaves it ready for the next.  Calls that share a workspace must not

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_rowq_kernel(const __
     }
     const uint32_t pos = __ldg(a.pos_start + seq) + j;
     unsigned long long row = 0;
-    const bool have_row = i1 > a.nh && rowq_row(a.cache, seq, pos, row);
+    const bool have_row = i1 > a.nh && pos >= j && rowq_row(a.cache, seq, pos, row);   // (pos < j: past 2^32)
     float cs[NP], sn[NP];
 #pragma unroll
     for (int p = 0; p < NP; ++p) { cs[p] = 1.f; sn[p] = 0.f; }
@@ -253,6 +253,7 @@ int launch_append_rowq(shady_ctx *ctx, const shady_append_params *p, const void 
     } else if (!total_tokens) {
         return SHADY_OK;
     }
+    if (const int st = pending_timeout(ctx, "kv_append_rowq")) return st;
     a.q = d_q; a.k = d_k; a.v = d_v; a.q_out = d_q_out; a.k_out = d_k_out; a.v_out = d_v_out; a.gate = d_gate;
     a.norm_w = norm_w; a.pos_start = d_pos_start; a.pos_h = d_pos_h; a.pos_w = d_pos_w; a.tok_start = d_tok_start;
     a.num_seqs = p->num_seqs; a.tokens_per_seq = p->tokens_per_seq; a.total_tokens = total_tokens;
@@ -317,9 +318,9 @@ __global__ void __launch_bounds__(kReadThreads) read_rowq_kernel(const __grid_co
     const uint32_t nr = min(a.rows_per_block, limit - r0);
     for (uint32_t r = warp; r < nr; r += kReadThreads / 32) {
         const uint32_t s = warp_find_seq(a.out_start, a.num_seqs, r0 + r, lane);
-        const uint32_t pos = (a.row_start ? __ldg(a.row_start + s) : 0u) + (r0 + r - __ldg(a.out_start + s));
+        const uint32_t j = r0 + r - __ldg(a.out_start + s), pos = (a.row_start ? __ldg(a.row_start + s) : 0u) + j;
         unsigned long long row = ~0ull;
-        if (!rowq_row(a.cache, s, pos, row)) row = ~0ull;
+        if (pos < j || !rowq_row(a.cache, s, pos, row)) row = ~0ull;   // (pos < j: past 2^32)
         if (lane == 0) sm_row[r] = row;
     }
     __syncthreads();
@@ -378,6 +379,7 @@ int launch_read_rowq(shady_ctx *ctx, const shady_rowq_cache *cache, uint32_t nkv
     ReadRowqArgs a{};
     if (const int st = fill_rowq_addr(ctx, cache, "kv_read_rowq", &a.cache)) return st;
     if (!total_rows) return SHADY_OK;
+    if (const int st = pending_timeout(ctx, "kv_read_rowq")) return st;
     a.row_start = d_row_start; a.out_start = d_out_start; a.k_out = d_k_out; a.v_out = d_v_out;
     a.num_seqs = num_seqs; a.total_rows = total_rows; a.nkv = nkv; a.hd = hd;
     // rows of a block: about 16 KB of codes of one tensor (128k rows of 8 heads of 128: 125 us; 32 KB 130, 64 KB 138), fewer

@@ -757,6 +757,7 @@ int launch_decode_rule(shady_ctx *ctx, const shady_decode_params *p, const shady
     }
     SHADY_REQUIRE(ctx, d_ws && ((uintptr_t)d_ws & 15) == 0 && ws_bytes >= dr::workspace_bytes(ctx, p), SHADY_ERR_WORKSPACE,
                   "decode_rule: workspace missing, unaligned or too small");
+    if (const int st = pending_timeout(ctx, "decode_rule")) return st;
     a.q = d_q; a.out = d_out; a.lse = d_lse; a.lens = d_seq_lens;
     a.records = reinterpret_cast<float *>(d_ws);
     a.group_counters = reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(d_ws) + dr::record_bytes(ctx));

@@ -234,7 +234,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if (s < a.num_seqs) {
                 qs = min(__ldg(a.q_starts + s), a.total_q);
                 T_s = max(min(__ldg(a.q_starts + s + 1), a.total_q), qs) - qs;
-                const uint32_t L = __ldg(a.kv_lens + s);
+                const uint32_t L = min(__ldg(a.kv_lens + s), 0x7fffff00u);
                 lo = L > T_s ? (L - T_s) / TPI : 0u;
                 hi = lo + (T_s + TPI - 1) / TPI;
             }

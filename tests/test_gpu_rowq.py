@@ -293,3 +293,22 @@ def test_refusals(gpu_ctx):
         with pytest.raises(ShadyError):
             ops.kv_read_rowq(gpu_ctx, **{**rd, **b})
     assert gpu_ctx.launch_count == n
+
+
+def test_positions_past_2_to_the_32_touch_no_row(gpu_ctx):
+    """A range that runs past the largest position ends there: it does not come round to row 0."""
+    c = Cache([8], 1, 64)
+    g = torch.Generator().manual_seed(5)
+    before = [t.clone() for t in (*c.codes, *c.scales)]
+    x = torch.randn(6, 1, 64, generator=g)
+    _, _, ko, _ = run_append(gpu_ctx, c, x, x, x, [0, 6], [2 ** 32 - 3], dt=F32, q_dt=F32, gate=False, norm=None, theta=1e4, rd=0, interleaved=True)
+    for a, b in zip((*c.codes, *c.scales), before):
+        assert torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0))
+    want_c, want_s = quantise(x)
+    assert torch.equal(ko.cpu(), (want_c.float() - 128) * want_s[..., None])
+    c.fill(0, [x, x])
+    out = torch.full((6, 1, 64), 7.0, device="cuda")
+    ops.kv_read_rowq(gpu_ctx, cache=c.view, k_out=out, row_start=dev_u32([2 ** 32 - 3]), out_start=dev_u32([0, 6]), total_rows=6, num_seqs=1,
+                     num_kv_heads=1, head_dim=64, out_dtype=F32)
+    gpu_ctx.synchronize()
+    assert bool((out == 0).all())

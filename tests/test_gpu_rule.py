@@ -600,3 +600,40 @@ def test_prefill_many_short_sequences_and_gaps(gpu_ctx):
     q_lens[5], q_lens[40], q_lens[69] = 3, 700, 0
     c = Rows16(kv_lens, 1, 128, BF16, "packed")
     check_prefill(gpu_ctx, c, c.values, q_lens, kv_lens, 1, 4, 128, BF16, dict(cap=25.0), heads=[0, 3])
+
+
+def test_launches_wait_for_an_uncollected_timeout(gpu_ctx):
+    """A wait of an earlier launch ran out and nobody has asked: the operators refuse until shady_synchronize has said so."""
+    from shady_thinker_b200._lib import ERR_TIMEOUT
+    from shady_thinker_b200.gpu import GpuContext
+    from shady_thinker_b200.p2p import ShardCombiner
+    gpu = GpuContext(0, stream=0x1)
+    gpu.set_wait_limits(peer_polls=1 << 12)
+    lone = ShardCombiner(gpu, rank=0, world=2, num_heads=8, head_dim=128, loopback=True)   # rank 1 does not exist
+    lone.combine(torch.zeros(8, 130, device="cuda"), torch.zeros(8, 128, device="cuda"))
+    torch.cuda.synchronize()
+    x = torch.ones(1, 2, 128, dtype=torch.float16, device="cuda")
+    codes, scales = torch.full((1, 2, 128), 128, dtype=torch.uint8, device="cuda"), torch.ones(1, 2, device="cuda")
+    rowq = ops.RowqCacheView(codes, codes, scales, scales, 1)
+    shape = dict(head_dim=128, num_kv_heads=2, num_q_heads=2, num_seqs=1)
+    n = ops.decode_rule_workspace_size(gpu, **shape)
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    one, span = dev_u32([1]), dev_u32([0, 1])
+    out = torch.empty_like(x)
+    calls = [lambda: ops.attn_decode_rule(gpu, q=x, cache=rowq, seq_lens=one, out=out, q_dtype=F16, out_dtype=F16, workspace=ws, workspace_bytes=n, **shape),
+             lambda: ops.attn_prefill_rule(gpu, q=x, cache=ops.KvCacheView(F16, x, x, 256), cache_rows=1, q_starts=span, total_q=1, kv_lens=one, out=out,
+                                           dtype=F16, **shape),
+             lambda: ops.kv_read_rowq(gpu, cache=rowq, k_out=out, out_start=span, total_rows=1, num_seqs=1, num_kv_heads=2, head_dim=128, out_dtype=F16),
+             lambda: ops.kv_append_rowq(gpu, q_proj_full=x, k_proj=x, v_proj=x, q_out=out, q_gate=None, cache=rowq, pos_start=one, num_heads=2,
+                                        num_kv_heads=2, head_dim=128, rope_theta=1e4, rotary_dim=0, has_gate=False, in_dtype=F16, q_dtype=F16)]
+    for call in calls:
+        with pytest.raises(ShadyError) as e:
+            call()
+        assert e.value.code == ERR_TIMEOUT
+    with pytest.raises(ShadyError):
+        gpu.synchronize()
+    for call in calls:
+        call()
+    gpu.synchronize()
+    lone.close()
+    gpu.close()
