@@ -134,6 +134,16 @@ __device__ __forceinline__ void cap_small(uint32_t &s0, uint32_t &s1, float c, f
     asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(p));
     s0 = __float_as_uint(y0); s1 = __float_as_uint(y1);
 }
+// The same for |s c| <= kTanhTiny, where two terms less do.
+__device__ __forceinline__ void cap_tiny(uint32_t &s0, uint32_t &s1, float c, float cap2, float add) {
+    const unsigned long long x = mul_f32x2(pack_f32x2(__uint_as_float(s0), __uint_as_float(s1)), both(c)), t = mul_f32x2(x, x);
+    unsigned long long p = fma2(t, both(kTanhT2 * cap2), both(kTanhT1 * cap2));
+    p = fma2(p, t, both(kTanhT0 * cap2));
+    p = fma2(p, x, both(add));
+    float y0, y1;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(p));
+    s0 = __float_as_uint(y0); s1 = __float_as_uint(y1);
+}
 // The same for all arguments: 1 - 2 / (1 + e^(2x)), one reciprocal for two elements; at an exponent of 60 the tanh is 1 to
 // the last bit, and the product of two sums still fits f32.
 __device__ __forceinline__ void cap_any(uint32_t &s0, uint32_t &s1, float c, float cap2, float add) {
@@ -508,8 +518,13 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                         for (uint32_t i = 0; i < 32; i += 2)
                             top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], fabsf(__uint_as_float(x[c][i])), fabsf(__uint_as_float(x[c][i + 1])));
-                    const bool small = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cap_c <= kTanhSmall;
-                    if (__all_sync(0xffffffffu, small)) {
+                    const float big = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * cap_c;
+                    if (__all_sync(0xffffffffu, big <= kTanhTiny)) {
+#pragma unroll
+                        for (uint32_t c = 0; c < N / 32; ++c)
+#pragma unroll
+                            for (uint32_t i = 0; i < 32; i += 2) cap_tiny(x[c][i], x[c][i + 1], cap_c, cap2, cap_add);
+                    } else if (__all_sync(0xffffffffu, big <= kTanhSmall)) {
 #pragma unroll
                         for (uint32_t c = 0; c < N / 32; ++c)
 #pragma unroll

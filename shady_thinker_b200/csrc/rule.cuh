@@ -46,6 +46,9 @@ __device__ __forceinline__ float rule_tanh_of_exp(float z2) { return 1.0f - 2.0f
 constexpr float kTanhSmall = 0.75f;
 constexpr float kTanhC0 = 0.999999821f, kTanhC1 = -0.333324701f, kTanhC2 = 0.133205801f, kTanhC3 = -0.0531492606f, kTanhC4 = 0.0192372371f,
                 kTanhC5 = -0.00449345633f;
+// the same for |x| <= 1/5 with P of degree 2: 1.0e-8, in f32 arithmetic 2.5e-8
+constexpr float kTanhTiny = 0.2f;
+constexpr float kTanhT0 = 0.999999643f, kTanhT1 = -0.333259940f, kTanhT2 = 0.129634932f;
 __device__ __forceinline__ float rule_tanh_small(float x) {
     const float t = x * x;
     return x * fmaf(fmaf(fmaf(fmaf(fmaf(kTanhC5, t, kTanhC4), t, kTanhC3), t, kTanhC2), t, kTanhC1), t, kTanhC0);
