@@ -5,13 +5,14 @@
 // decode_rule.cu, over the rows j that the rule lets position i see (shady_score_rule).
 //
 // What bounds it: 4 hd operations per (query head, visible row) on the tensor pipe against one exponential on the special
-// function unit, which runs 16 per clock and SM, and with a cap nine two-lane multiply-adds per pair of elements on an FMA
-// pipe that takes two clocks for each.  A 128 x 64 tile of head_dim 128 owes the tensor pipe 768 clocks (its N = 64 score
-// MMAs run at half rate), the exponentials 512, a cap 576 of the FMA pipe; stamps put a tile at about 1,150 clocks without a
-// rule and 1,450 with a cap, the rest being the latencies of one warp per scheduler and row tile.
-// Measured (B200, bf16): 4 x 4096 tokens, 32 heads of 128 over 8, cap 50: 0.79 ms = 697 TFLOP/s, no cap 0.64 ms = 865;
-// 8,192 tokens of packed documents behind a window of 2,048: 0.116 ms; 2 x 1024 tokens behind 8,192 rows, head_dim 256,
-// distance bias: 0.168 ms = 880 TFLOP/s; seven prompts of up to 301 tokens, capped: 15.6 us.
+// function unit, which runs 16 per clock and SM, and with a cap five (scores beyond a fifth of the cap: eight) two-lane
+// multiply-adds per pair of elements on an FMA pipe that takes two clocks for each.  A 128 x 64 tile of head_dim 128 owes the
+// tensor pipe about 850 clocks (a score MMA with N = 64 takes 70 of them instead of 32: its A tile comes from shared memory
+// at 128 bytes per clock), the exponentials 512, a cap 320 of the FMA pipe; stamps put a tile at about 900 clocks without a
+// rule and 1,100 with a cap, where two warps per scheduler share one FMA pipe and one special function unit.
+// Measured (B200, bf16): 4 x 4096 tokens, 32 heads of 128 over 8, cap 50: 0.70 ms = 785 TFLOP/s, no cap 0.55..0.61 ms =
+// 900..1,010; 8,192 tokens of packed documents behind a window of 2,048: 0.114 ms; 2 x 1024 tokens behind 8,192 rows,
+// head_dim 256, distance bias: 0.143 ms = 1,030 TFLOP/s; seven prompts of up to 301 tokens, f16, capped: 15.4 us.
 //
 //   * The query heads of a kv head share a row tile: row r of a tile is token r / G, head r % G (G heads per kv head,
 //     128 / G whole tokens per tile).  K and V are then fetched once for all of them, a chunk of a few tokens fills a
@@ -24,11 +25,13 @@
 //     ring in shared memory.
 //   * K and V tiles of 64 rows come through rings of their own (a K slot is free once its scores are computed); rows past
 //     a sequence's end may hold anything, so they are cleared in the V tile (0 * NaN) before the MMA.
-//   * Scores are issued up to kNS tiles ahead into buffers of their own, so that the softmax does not wait for its P's
-//     product (with two row tiles and one 128-column buffer each it idled 2,100 of 6,200 clocks).
+//   * The softmax threads take a score tile to registers whole, which frees its TMEM columns for the next tile's scores at
+//     once, and write the weights to columns of their own, twice as many as a tile needs.  So neither product waits for the
+//     other's (weights written over their scores left the softmax idle for half of every 2,300 clocks).
+//   * Two threads issue scores and one the PVs, one warp finds the items and requests the rows.
 //   * Softmax, one thread per row: the tile's scores are taken to registers whole, transformed, masked by 32-bit words that
-//     interval arithmetic gives (skipped by a warp whose rows see the whole tile), and P goes back over S as the A operand
-//     of the second MMA.  O is only rescaled when a row's maximum grew by more than 2^8.
+//     interval arithmetic gives (skipped by a warp whose rows see the whole tile), and P goes to TMEM as the A operand of the
+//     second MMA.  O is only rescaled when a row's maximum grew by more than 2^8.
 // Every wait is bounded (see shady_ctx_set_wait_limits).
 #include <cuda.h>
 
@@ -48,7 +51,7 @@ struct Args {
     void *out;
     float *lse;
     const uint32_t *page_table;
-    uint32_t page_rows, max_pages, box_rows;
+    uint32_t page_rows, max_pages, box_rows, box_slabs;
     unsigned long long seq_rows;
     const uint32_t *q_starts, *kv_starts, *kv_lens;
     uint32_t num_seqs, total_q, nkv, nh, G;
@@ -57,21 +60,23 @@ struct Args {
 template <int HD> struct Cfg {
     static constexpr uint32_t kNT = HD == 128 ? 2 : 1;          // row tiles of an item
     static constexpr uint32_t kN = 64;                          // K/V rows of a tile
-    static constexpr uint32_t kNS = HD == 128 ? 2 : 3;          // score buffers of a row tile: scores are issued that many tiles ahead
+    static constexpr uint32_t kNS = HD == 128 ? 1 : 2;          // score buffers of a row tile
+    static constexpr uint32_t kNP = HD == 128 ? 2 : 3;          // weight buffers of a row tile
     static constexpr uint32_t kSlabs = HD / 64;                 // 64-element (128-byte) slabs of a row
     static constexpr uint32_t kKvSlab = kN * 128, kKvTile = kSlabs * kKvSlab;
     static constexpr uint32_t kQSlab = 128 * 128, kQTile = kSlabs * kQSlab;
     static constexpr uint32_t kKS = HD == 128 ? 5 : 3, kVS = HD == 128 ? 5 : 2;   // slots of the K and V rings
     static constexpr uint32_t kSmemK = kNT * kQTile, kSmemV = kSmemK + kKS * kKvTile, kSmemMisc = kSmemV + kVS * kKvTile;
     static constexpr uint32_t kSmem = kSmemMisc + 768 + 1024;   // barriers, item ring; slack for 1024-byte alignment
-    static constexpr uint32_t kColO = 256;                      // TMEM: scores of row tile q, buffer b at 64 (q kNS + b), O_q at 256 + 128 q
+    // TMEM columns: per row tile its score buffers (64 f32 each), then its weight buffers (64 16-bit values, 32 columns); O behind all
+    static constexpr uint32_t kColP = kNS * kN, kColTile = kColP + kNP * kN / 2, kColO = 256;
     static constexpr uint32_t kThreads = kNT * 128 + 128;
     static_assert(kSmem <= 232448, "Q and the rings must fit in 227 KB");
-    static_assert(kNT * kNS * kN <= kColO && kColO + kNT * HD <= 512, "TMEM columns");
+    static_assert(kNT * kColTile <= kColO && kColO + kNT * HD <= 512, "TMEM columns");
 };
 constexpr uint32_t kItems = 4;   // slots of the item ring
 enum { B_IFULL = 0, B_IEMPTY = B_IFULL + kItems, B_QFULL = B_IEMPTY + kItems, B_QEMPTY = B_QFULL + 2, B_KFULL = B_QEMPTY + 2, B_KEMPTY = B_KFULL + 5,
-       B_VFULL = B_KEMPTY + 5, B_VEMPTY = B_VFULL + 5, B_SFULL = B_VEMPTY + 5, B_PFULL = B_SFULL + 4, B_PVDONE = B_PFULL + 4, B_OFULL = B_PVDONE + 4,
+       B_VFULL = B_KEMPTY + 5, B_VEMPTY = B_VFULL + 5, B_SFULL = B_VEMPTY + 5, B_SFREE = B_SFULL + 2, B_PFULL = B_SFREE + 2, B_PVDONE = B_PFULL + 4, B_OFULL = B_PVDONE + 4,
        B_TURN = B_OFULL + 2, B_COUNT = B_TURN + 2 };
 constexpr uint32_t kItemOff = 8 * B_COUNT + 16;   // item descriptors of 16 words behind the barriers, the TMEM slot and the abort word
 static_assert(kItemOff + kItems * 64 <= 768, "barriers and item ring");
@@ -84,13 +89,13 @@ struct Item {
     uint32_t pre;                  // prefix rows
     // Tile j of the item.  With a distance bias the last one comes first: the scores fall from there on, so the running maximum
     // settles at once (first to last it grew by more than the threshold with every tile, and O was rescaled each time: 231 us
-    // of the head_dim 256 chunk against 165).  Without one the order that ends with the masked tiles is a little faster.
+    // of the head_dim 256 chunk against 165 then).  Without one the order that ends with the masked tiles is a little faster.
     template <bool REV> __device__ __forceinline__ uint32_t tile(uint32_t j) const {
         if (REV) j = n - 1 - j;
         return j < na ? a0 + j : b0 + (j - na);
     }
 };
-__device__ __forceinline__ Item item_read(const volatile uint32_t *w) {
+template <typename W> __device__ __forceinline__ Item item_of(const W &w) {
     Item it;
     it.valid = w[0]; it.seq = w[1]; it.kvh = w[2]; it.tok0 = w[3]; it.ntok = w[4]; it.pos0 = (int32_t)w[5]; it.L = w[6]; it.row0 = w[7];
     it.a0 = w[8]; it.na = w[9]; it.b0 = w[10]; it.n = w[11]; it.pre = w[12];
@@ -101,6 +106,10 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
     lo = max(lo, 0); hi = min(hi, 32);
     if (lo >= hi) return 0u;
     return (hi == 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2, int c3, int c4) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4) : "memory");
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -158,14 +167,14 @@ __device__ __forceinline__ void cap_any(uint32_t &s0, uint32_t &s1, float c, flo
 // MODE 0: scale only, 1: tanh cap, 2: distance bias, with or without a cap; 3: tanh cap with a fixed reference.
 // A cap bounds y = z log2(e) by +-cap2, and bf16 weights have the range of f32: with cap2 <= kFixedCap the weights are
 // 2^(y - cap2/2), between 2^(-3/2 cap2) and 2^(cap2/2), and neither a row maximum nor a rescaling of O is needed (4 x 4096
-// batch, cap 50: 788 us, with a running maximum 887).
+// batch, cap 50: 700 us, with a running maximum 775).
 constexpr float kFixedCap = 80.0f;
 template <typename T, int HD, int MODE>
 __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
 prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ Args a) {
     using C = Cfg<HD>;
-    constexpr uint32_t NT = C::kNT, N = C::kN, NS = C::kNS;
+    constexpr uint32_t NT = C::kNT, N = C::kN, NS = C::kNS, NP = C::kNP, kLead = NS + 1;   // kLead: K tiles in front of V
     constexpr bool kRev = MODE == 2;
     constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     extern __shared__ unsigned char smem_raw[];
@@ -179,21 +188,22 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (gave_up(a.status)) return;
     const WaitCtx wc{abort_word, a.status, a.wait_mbar};
-    constexpr uint32_t kWProd = 4 * NT, kWMma = kWProd + 1, kWSched = kWProd + 2, kWPv = kWProd + 3;
+    constexpr uint32_t kWProd = 4 * NT, kWScore = kWProd + 1, kWPv = kWProd + 3;   // (two warps issue scores)
     const uint32_t TPT = 128u / a.G, R = TPT * a.G, TPI = NT * TPT;   // tokens and rows of a tile, tokens of an item
 
     if (warp == kWProd && lane == 0) {
         for (uint32_t i = 0; i < kItems; ++i) {
             mbar_init(bar(B_IFULL + i), 1);
-            mbar_init(bar(B_IEMPTY + i), 3 + 4 * NT);   // producer, two issuers, softmax warps
+            mbar_init(bar(B_IEMPTY + i), 3 + 4 * NT);   // issuers and softmax warps
         }
         for (uint32_t i = 0; i < 2; ++i) {
-            mbar_init(bar(B_QFULL + i), 1); mbar_init(bar(B_QEMPTY + i), 1); mbar_init(bar(B_OFULL + i), 1);
+            mbar_init(bar(B_QFULL + i), 1); mbar_init(bar(B_QEMPTY + i), 3 - NT); mbar_init(bar(B_OFULL + i), 1);
             mbar_init(bar(B_TURN + i), 128);
         }
-        for (uint32_t i = 0; i < C::kKS; ++i) { mbar_init(bar(B_KFULL + i), 1); mbar_init(bar(B_KEMPTY + i), 1); }
+        for (uint32_t i = 0; i < C::kKS; ++i) { mbar_init(bar(B_KFULL + i), 1); mbar_init(bar(B_KEMPTY + i), NT); }
         for (uint32_t i = 0; i < C::kVS; ++i) { mbar_init(bar(B_VFULL + i), 1); mbar_init(bar(B_VEMPTY + i), 1); }
-        for (uint32_t i = 0; i < NT * NS; ++i) { mbar_init(bar(B_SFULL + i), 1); mbar_init(bar(B_PFULL + i), 128); mbar_init(bar(B_PVDONE + i), 1); }
+        for (uint32_t i = 0; i < NT * NS; ++i) { mbar_init(bar(B_SFULL + i), 1); mbar_init(bar(B_SFREE + i), 128); }
+        for (uint32_t i = 0; i < NT * NP; ++i) { mbar_init(bar(B_PFULL + i), 128); mbar_init(bar(B_PVDONE + i), 1); }
         *abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -207,7 +217,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == kWMma) {
+    if (warp == kWScore) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -220,7 +230,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     // one of a whole warp differ in who says that the slot has been read.
     auto take_item = [&](uint32_t ic, Item &it, auto whole_warp, int code) {
         if (!mbar_wait(bar(B_IFULL + ic % kItems), (ic / kItems) & 1, wc, code)) return false;
-        it = item_read(items + 16 * (ic % kItems));
+        it = item_of(items + 16 * (ic % kItems));
         if constexpr (decltype(whole_warp)::value) __syncwarp();
         if (!decltype(whole_warp)::value || lane == 0) mbar_arrive(bar(B_IEMPTY + ic % kItems));
         return it.valid != 0;
@@ -229,12 +239,12 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     constexpr std::false_type kThreadRole{};
 
     if (warp >= kWProd) {
-    if (warp == kWSched) {
-        // =============================== items ===============================
+    if (warp == kWProd) {
+        // =============================== items, TMA producer ===============================
         // 32 sequences at a time, one per lane.  A sequence's blocks stand at levels [lo, hi) = their first position / TPI; the
         // list runs from the highest level down (the blocks with the most rows in front of them first, so that the list
         // ends with small items), at one level over the sequences that have a block there, for each over the kv heads.
-        uint32_t chunk = 0, ic = 0;
+        uint32_t chunk = 0, rnd = 0;
         uint32_t qs = 0, T_s = 0, lo = 0, hi = 0;
         unsigned long long base = 0, w = 0;   // items in front of `level`; the item wanted
         uint32_t level = 0;                   // levels above it are done; 0: none left in this chunk
@@ -251,9 +261,11 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             level = __reduce_max_sync(0xffffffffu, T_s ? hi : 0u);
         };
         load_chunk();
-        bool ok = true, more = true;
-        for (uint32_t rnd = 0; more && ok; ++rnd, ++ic) {
+        bool ok = true;
+        // the next item, or the end of the list, into its slot of the ring (the whole warp); false: a wait gave up
+        auto next_item = [&](Item &it) {
             w = (unsigned long long)rnd * gridDim.x + ((rnd & 1u) ? gridDim.x - 1u - blockIdx.x : blockIdx.x);
+            bool more = true;
             uint32_t active = 0;   // sequences with a block at level - 1
             while (true) {
                 if (!level) {
@@ -311,70 +323,89 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                 for (int i = 0; i < 13; ++i) vals[i] = v[i];
             }
-            if (ic >= kItems) ok = mbar_wait(bar(B_IEMPTY + ic % kItems), (ic / kItems - 1) & 1, wc, 31);
-            if (!ok) break;
+            const bool free_slot = rnd < kItems || mbar_wait(bar(B_IEMPTY + rnd % kItems), (rnd / kItems - 1) & 1, wc, 31);
+            if (!__all_sync(0xffffffffu, free_slot)) return false;
             if (lane == 0) {
 #pragma unroll
-                for (int i = 0; i < 13; ++i) items[16 * (ic % kItems) + i] = vals[i];
-                mbar_arrive(bar(B_IFULL + ic % kItems));
+                for (int i = 0; i < 13; ++i) items[16 * (rnd % kItems) + i] = vals[i];
+                mbar_arrive(bar(B_IFULL + rnd % kItems));
             }
             __syncwarp();
-        }
-    } else if (warp == kWProd) {
-        // =============================== TMA producer ===============================
-        if (lane == 0) {
-            bool ok = true;
-            uint32_t gk = 0, gv = 0, qn[2] = {0, 0};   // K and V tiles, Q tiles of each row tile requested so far
-            Item it{};
-            auto load_kv = [&](uint32_t dst, const CUtensorMap *map, uint32_t b, uint32_t k0) {
-                if (a.page_table) {
-                    for (uint32_t r = 0; r < N; r += a.box_rows) {   // a box never leaves its page; past the sequence: a page that does not exist reads as zero
-                        const uint32_t row = k0 + r, pi = row / a.page_rows;
-                        const int page = row < it.L && pi < a.max_pages ? (int)__ldg(a.page_table + (size_t)it.seq * a.max_pages + pi) : -1;
-#pragma unroll
-                        for (uint32_t c = 0; c < C::kSlabs; ++c)
-                            tma_load_4d(dst + c * C::kKvSlab + r * 128u, map, b, 64 * c, (int)it.kvh, (int)(row % a.page_rows), page);
+            it = item_of(vals);
+            ++rnd;
+            return true;
+        };
+        uint32_t gk = 0, gv = 0, qn[2] = {0, 0};   // K and V tiles, Q tiles of each row tile requested so far
+        Item it{}, ahead{};
+        auto wait_all = [&](uint32_t b, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(b, parity, wc, code)) != 0; };
+        // A request is one box: the whole tile, or where a tile spans pages a 64-element slab of the rows that lie on one page, each
+        // by a lane of its own.  The lanes find the rows and pages of the next 32 boxes together (two divisions and a lookup for
+        // every tile, and a request per slab, kept head_dim 256 waiting for its rows: 202 us of the chunk against 143).
+        const uint32_t box_rows = a.box_rows, boxes = N / box_rows, b_shift = 31 - __clz(boxes);   // boxes of rows in a tile: a power of two
+        const bool whole = a.box_slabs > 1;
+        const uint32_t box = whole ? lane : lane / C::kSlabs, slab = whole ? 0u : lane % C::kSlabs;
+        const uint32_t to = slab * C::kKvSlab + box * box_rows * 128u;
+        struct Where { int page, row; };
+        auto load_kv = [&](uint32_t dst, const CUtensorMap *map, uint32_t b, uint32_t j, Where &w) {
+            if (lane == 0) mbar_expect_tx(b, C::kKvTile);
+            const uint32_t first = (j << b_shift) & 31;   // the lane that found this tile's first box
+            if (!first) {
+                const uint32_t jj = j + (lane >> b_shift);
+                w = Where{-1, 0};   // past the sequence: a page that does not exist reads as zero
+                if (jj < it.n) {
+                    const uint32_t row = it.template tile<kRev>(jj) * N + (lane & (boxes - 1)) * box_rows;
+                    if (a.page_table) {
+                        const uint32_t pi = row / a.page_rows;
+                        w.row = (int)(row - pi * a.page_rows);
+                        if (row < it.L && pi < a.max_pages) w.page = (int)__ldg(a.page_table + (size_t)it.seq * a.max_pages + pi);
+                    } else {
+                        w = Where{0, (int)(it.row0 + row)};
                     }
-                } else {
-#pragma unroll
-                    for (uint32_t c = 0; c < C::kSlabs; ++c) tma_load_4d(dst + c * C::kKvSlab, map, b, 64 * c, (int)it.kvh, (int)(it.row0 + k0), 0);
                 }
-            };
-            auto load_k = [&](uint32_t j) {
-                const uint32_t s = gk % C::kKS;
-                if (gk >= C::kKS && !mbar_wait(bar(B_KEMPTY + s), (gk / C::kKS - 1) & 1, wc, 32)) return false;
-                mbar_expect_tx(bar(B_KFULL + s), C::kKvTile);
-                load_kv(smem_base + C::kSmemK + s * C::kKvTile, &map_k, bar(B_KFULL + s), it.template tile<kRev>(j) * N);
-                ++gk;
-                return true;
-            };
-            auto load_v = [&](uint32_t j) {
-                const uint32_t s = gv % C::kVS;
-                if (gv >= C::kVS && !mbar_wait(bar(B_VEMPTY + s), (gv / C::kVS - 1) & 1, wc, 33)) return false;
-                mbar_expect_tx(bar(B_VFULL + s), C::kKvTile);
-                load_kv(smem_base + C::kSmemV + s * C::kKvTile, &map_v, bar(B_VFULL + s), it.template tile<kRev>(j) * N);
-                ++gv;
-                return true;
-            };
-            for (uint32_t ic = 0; ok && take_item(ic, it, kThreadRole, 34); ++ic) {
-                if (!it.n) continue;
+            }
+            const int page = __shfl_sync(0xffffffffu, w.page, first + box), row = __shfl_sync(0xffffffffu, w.row, first + box);
+            if (box < boxes) tma_load_5d(dst + to, map, b, 0, row, (int)slab, (int)it.kvh, page);
+        };
+        Where at_k{}, at_v{};
+        auto load_k = [&](uint32_t j) {
+            const uint32_t s = gk % C::kKS;
+            if (gk >= C::kKS && !wait_all(bar(B_KEMPTY + s), (gk / C::kKS - 1) & 1, 32)) return false;
+            load_kv(smem_base + C::kSmemK + s * C::kKvTile, &map_k, bar(B_KFULL + s), j, at_k);
+            ++gk;
+            return true;
+        };
+        auto load_v = [&](uint32_t j) {
+            const uint32_t s = gv % C::kVS;
+            if (gv >= C::kVS && !wait_all(bar(B_VEMPTY + s), (gv / C::kVS - 1) & 1, 33)) return false;
+            load_kv(smem_base + C::kSmemV + s * C::kKvTile, &map_v, bar(B_VFULL + s), j, at_v);
+            ++gv;
+            return true;
+        };
+        // The item after this one is worked out behind this one's first requests.
+        ok = next_item(it);
+        while (ok && it.valid) {
+            if (it.n) {
                 ok = load_k(0);   // ahead of Q, which waits for the last scores of the item before
                 for (uint32_t q = 0; q < NT && ok; ++q) {
                     if (q * TPT >= it.ntok) continue;
-                    if (qn[q] > 0) ok = mbar_wait(bar(B_QEMPTY + q), (qn[q] - 1) & 1, wc, 35);
+                    if (qn[q] > 0) ok = wait_all(bar(B_QEMPTY + q), (qn[q] - 1) & 1, 35);
                     if (!ok) break;
                     ++qn[q];
-                    mbar_expect_tx(bar(B_QFULL + q), C::kSlabs * R * 128u);
-#pragma unroll
-                    for (uint32_t c = 0; c < C::kSlabs; ++c)
-                        tma_load_3d(smem_base + q * C::kQTile + c * C::kQSlab, &map_q, bar(B_QFULL + q), 64 * c, (int)(it.kvh * a.G), (int)(it.tok0 + q * TPT));
-                }
-                // K runs in front of V, as the score MMAs run in front of the PV MMAs
-                for (uint32_t j = 1; j < it.n + NS && ok; ++j) {
-                    if (j < it.n) ok = load_k(j);
-                    if (ok && j >= NS) ok = load_v(j - NS);
+                    if (lane == 0) mbar_expect_tx(bar(B_QFULL + q), C::kSlabs * R * 128u);
+                    __syncwarp();
+                    if (lane < C::kSlabs)
+                        tma_load_3d(smem_base + q * C::kQTile + lane * C::kQSlab, &map_q, bar(B_QFULL + q), 64 * lane, (int)(it.kvh * a.G), (int)(it.tok0 + q * TPT));
                 }
             }
+            ok = ok && next_item(ahead);
+            // K runs in front of V, as the score MMAs run in front of the PV MMAs
+            for (uint32_t j = 1; ok && it.n && j < it.n + kLead; ++j) {
+                if (j < it.n) ok = load_k(j);
+                if (ok && j >= kLead) ok = load_v(j - kLead);
+            }
+            it = ahead;
+        }
+        if (lane == 0) {
             if (*abort_word || gave_up(a.status)) {   // copies may be in flight: a bounded time for them to land before the memory is handed back
                 for (uint32_t s = 0; s < C::kKS; ++s)
                     for (uint32_t i = 0; gk > s && i < (1u << 16) && !mbar_try(bar(B_KFULL + s), ((gk - 1 - s) / C::kKS) & 1); ++i) {}
@@ -384,36 +415,42 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     for (uint32_t i = 0; qn[q] && i < (1u << 16) && !mbar_try(bar(B_QFULL + q), (qn[q] - 1) & 1); ++i) {}
             }
         }
-    } else if (warp == kWMma) {
+    } else if (warp < kWPv) {
         // =============================== score MMAs ===============================
-        // Scores and PVs are issued by a thread each: a satisfied wait costs a thread some 250 clocks and a commit 80, and together
-        // they add up to twice what the tensor pipe needs for a tile of 64 rows.  MMAs of different threads are not ordered, so
-        // a score buffer is only overwritten once the PV that read P from it is complete.
+        // Two threads issue scores, a row tile each or every other tile of the one, and one the PVs: a satisfied wait costs a
+        // thread some 250 clocks and a commit 80, and one thread for all scores took 2,330 clocks a pair of tiles, 1,150 of
+        // them issuing (4 x 4096 batch without a cap 655 us, with two threads 590).  A score buffer is free as soon as the
+        // softmax threads have it in registers.
         if (lane == 0) {
-            const uint32_t idesc = make_idesc(kFmt, false, N);
+            const uint32_t idesc = make_idesc(kFmt, false, N), me = warp - kWScore, q = NT == 2 ? me : 0u;
+            const uint32_t qa = smem_base + q * C::kQTile;
             bool ok = true;
-            uint32_t gk = 0, qn[2] = {0, 0}, qc[2] = {0, 0};   // K and Q tiles, score tiles of each row tile so far
+            uint32_t gk = 0, qn = 0, t = 0;   // K tiles, Q tiles and score tiles so far
             Item it{};
             for (uint32_t ic = 0; ok && take_item(ic, it, kThreadRole, 41); ++ic) {
-                const uint32_t n = it.n, nq = NT == 2 && it.ntok > TPT ? 2u : 1u;
-                for (uint32_t j = 0; j < n && ok; ++j, ++gk) {
-                    for (uint32_t q = 0; q < nq; ++q) {
-                        if (j == 0 && !(ok = mbar_wait(bar(B_QFULL + q), qn[q]++ & 1, wc, 42))) break;
-                        if (q == 0 && !(ok = mbar_wait(bar(B_KFULL + gk % C::kKS), (gk / C::kKS) & 1, wc, 38))) break;
-                        const uint32_t t = qc[q]++, b = q * NS + t % NS;
-                        if (t >= NS && !(ok = mbar_wait(bar(B_PVDONE + b), (t / NS - 1) & 1, wc, 43))) break;
-                        tc_fence_after();
-                        const uint32_t qa = smem_base + q * C::kQTile, kb = smem_base + C::kSmemK + (gk % C::kKS) * C::kKvTile;
-#pragma unroll
-                        for (uint32_t ks = 0; ks < HD / 16; ++ks) {
-                            const uint32_t so = ks >> 2, ko = (ks & 3) * 32;
-                            mma_ss(tmem + b * N, desc_kmajor(qa + so * C::kQSlab + ko), desc_kmajor(kb + so * C::kKvSlab + ko), idesc, ks > 0);
-                        }
-                        tc_commit(bar(B_SFULL + b));
-                        if (q + 1 == nq) tc_commit(bar(B_KEMPTY + gk % C::kKS));
-                        if (j == n - 1) tc_commit(bar(B_QEMPTY + q));
+                if (!it.n) continue;
+                const bool have = q * TPT < it.ntok;
+                if (have && !(ok = mbar_wait(bar(B_QFULL + q), qn++ & 1, wc, 42))) break;
+                for (uint32_t j = 0; j < it.n; ++j, ++gk, t += have) {
+                    const uint32_t ks = gk % C::kKS, b = q * NS + t % NS;
+                    if (NT == 1 && (gk & 1u) != me) continue;   // the other thread's
+                    if (!(ok = mbar_wait(bar(B_KFULL + ks), (gk / C::kKS) & 1, wc, 38))) break;
+                    if (!have) {   // this row tile is empty
+                        mbar_arrive(bar(B_KEMPTY + ks));
+                        continue;
                     }
+                    if (t >= NS && !(ok = mbar_wait(bar(B_SFREE + b), (t / NS - 1) & 1, wc, 43))) break;
+                    tc_fence_after();
+                    const uint32_t kb = smem_base + C::kSmemK + ks * C::kKvTile;
+#pragma unroll
+                    for (uint32_t k = 0; k < HD / 16; ++k) {
+                        const uint32_t so = k >> 2, ko = (k & 3) * 32;
+                        mma_ss(tmem + q * C::kColTile + t % NS * N, desc_kmajor(qa + so * C::kQSlab + ko), desc_kmajor(kb + so * C::kKvSlab + ko), idesc, k > 0);
+                    }
+                    tc_commit(bar(B_SFULL + b));
+                    tc_commit(bar(B_KEMPTY + ks));
                 }
+                if (ok && have) tc_commit(bar(B_QEMPTY + q));   // (a thread without a tile here arrives at once)
             }
         }
     } else if (warp == kWPv) {
@@ -441,14 +478,14 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     __syncwarp();
                 }
                 for (uint32_t q = 0; q < nq; ++q) {
-                    const uint32_t t = qc[q]++, b = q * NS + t % NS;
+                    const uint32_t t = qc[q]++, b = q * NP + t % NP;
                     // (a softmax thread reads O of the item before ahead of its arrival here, so the first tile may overwrite it)
-                    if (!(ok = mbar_wait(bar(B_PFULL + b), (t / NS) & 1, wc, 45))) break;
+                    if (!(ok = mbar_wait(bar(B_PFULL + b), (t / NP) & 1, wc, 45))) break;
                     tc_fence_after();
                     if (lane == 0) {
 #pragma unroll
                         for (uint32_t ks = 0; ks < N / 16; ++ks)
-                            mma_ts(tmem + C::kColO + q * 128, tmem + b * N + ks * 8, desc_mnmajor(smem_base + vt + ks * 2048, C::kKvSlab), idesc, j > 0 || ks > 0);
+                            mma_ts(tmem + C::kColO + q * 128, tmem + q * C::kColTile + C::kColP + t % NP * (N / 2) + ks * 8, desc_mnmajor(smem_base + vt + ks * 2048, C::kKvSlab), idesc, j > 0 || ks > 0);
                         tc_commit(bar(B_PVDONE + b));
                         if (q + 1 == nq) tc_commit(bar(B_VEMPTY + gv % C::kVS));
                         if (j == n - 1) tc_commit(bar(B_OFULL + q));
@@ -499,17 +536,20 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if (MODE == 2) slope2 = live ? __ldg(a.rule.slopes + slot[2] * a.G + g) * kRuleLog2e : 0.f;
             float m_ref = MODE == 3 ? 0.5f * cap2 : -INFINITY, l_sum = 0.f;
             for (uint32_t j = 0; j < n && ok; ++j, k0 = j == turn ? (int32_t)(other * N) : (kRev ? k0 - (int32_t)N : k0 + (int32_t)N)) {
-                const uint32_t b = q * NS + cnt % NS;
-                ok = mbar_wait(bar(B_SFULL + b), (cnt / NS) & 1, wc, 47);
+                const uint32_t b = q * NS + cnt % NS, pb = q * NP + cnt % NP;
+                // the weights' buffer first: the product that read it, kNP tiles back, is done by now, and scores are still to come
+                ok = (cnt < NP || mbar_wait(bar(B_PVDONE + pb), (cnt / NP - 1) & 1, wc, 40)) && mbar_wait(bar(B_SFULL + b), (cnt / NS) & 1, wc, 47);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t t_s = t_lane + b * N;
+                const uint32_t t_s = t_lane + q * C::kColTile + cnt % NS * N;
                 uint32_t x[N / 32][32];
 #pragma unroll
                 for (uint32_t c = 0; c < N / 32; ++c) tmem_ld32(t_s + c * 32, x[c]);
                 // (a row without a token may hold and become anything)
                 const bool whole = !live || (c_lo <= k0 && c_hi >= k0 + (int32_t)N) || (p_lo <= k0 && p_hi >= k0 + (int32_t)N);
                 tmem_wait_ld();
+                tc_fence_before();
+                mbar_arrive(bar(B_SFREE + b));
                 // ---- the rule: x = z log2(e), or with scale alone the raw product ----
                 if (MODE == 1 || MODE == 3 || (MODE == 2 && a.rule.cap > 0.f)) {
                     float top[4] = {0.f, 0.f, 0.f, 0.f};
@@ -589,7 +629,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     }
                     if (__any_sync(0xffffffffu, corr != 1.f)) {
                         // the PV of the tile before must have written O (its buffer's own barrier: the PVs of several tiles may be under way)
-                        ok = mbar_wait(bar(B_PVDONE + q * NS + (cnt - 1) % NS), ((cnt - 1) / NS) & 1, wc, 48);
+                        ok = mbar_wait(bar(B_PVDONE + q * NP + (cnt - 1) % NP), ((cnt - 1) / NP) & 1, wc, 48);
                         if (!ok) break;
                         tc_fence_after();
                         l_sum *= corr;
@@ -606,15 +646,19 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 }
                 // The two row tiles' scores come together, and both warpgroups would transform them on the FMA pipe and then both
                 // exponentiate on the special function unit.  Taking turns at the exponentials sets them half a tile apart, so
-                // that each pipe is in use throughout.
-                const bool turns = NT == 2 && (MODE == 1 || MODE == 3 || (MODE == 2 && a.rule.cap > 0.f)) && ntok > TPT;
+                // that each pipe is in use throughout (cap 50, 4 x 2048 tokens: 182 us, without turns 198; with a distance bias too 235
+                // and 248).  With a running maximum and no bias it only pays where there are few tiles (f16, cap 50, seven prompts
+                // of up to 301 tokens 15.4 and 16.2 us, but 4 x 2048 tokens 221 and 212).
+                const bool capped = MODE == 1 || MODE == 3 || (MODE == 2 && a.rule.cap > 0.f);
+                const bool turns = NT == 2 && capped && (MODE != 1 || n <= 16) && ntok > TPT;
                 if (turns) {
                     if (q == 0) ok = tc == 0 || mbar_wait(bar(B_TURN), (tc - 1) & 1, wc, 36);
                     else ok = mbar_wait(bar(B_TURN + 1), tc & 1, wc, 37);
                     if (!ok) break;
                     ++tc;
                 }
-                // ---- P = 2^(x - m), row sum, packed over S ----
+                // ---- P = 2^(x - m) and the row sum ----
+                const uint32_t t_p = t_lane + q * C::kColTile + C::kColP + cnt % NP * (N / 2);
                 const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref;   // nothing seen yet: every weight is 2^-inf
                 const float mul = MODE == 0 ? scale2 : 1.0f;
                 const unsigned long long mul2 = pack_f32x2(mul, mul), negm2 = pack_f32x2(neg_m, neg_m);
@@ -631,7 +675,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         ls2[(i >> 1) & 1] = add_f32x2(ls2[(i >> 1) & 1], pack_f32x2(p0, p1));
                         pk[i >> 1] = pack16<T>(p0, p1);
                     }
-                    tmem_st16(t_s + c * 16, pk);
+                    tmem_st16(t_p + c * 16, pk);
                 }
                 if (turns) mbar_arrive(bar(B_TURN + 1 - q));
                 float s0, s1, s2, s3;
@@ -640,7 +684,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 l_sum += (s0 + s1) + (s2 + s3);
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(bar(B_PFULL + b));
+                mbar_arrive(bar(B_PFULL + pb));
                 ++cnt;
             }
             // ---- epilogue: O / l, lse ----
@@ -683,7 +727,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     // ---- teardown: everyone arrives, TMEM goes back ----
     tc_fence_before();
     __syncthreads();
-    if (warp == kWMma) {
+    if (warp == kWScore) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
@@ -702,7 +746,7 @@ static EncodeFn encode_fn() {
     return fn;
 }
 static bool encode(CUtensorMap *map, uint32_t dtype, const void *base, uint32_t rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
-    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
     EncodeFn fn = encode_fn();
     return fn && fn(map, dtype == SHADY_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(base), dims,
                     strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -776,10 +820,12 @@ int launch_prefill_rule(shady_ctx *ctx, const shady_prefill_params *p, const sha
         uint32_t rows = tile;   // rows of a box: a tile, or the largest power of two that divides both a tile and a page
         while (kv.page_table && kv.page_rows % rows) rows /= 2;
         a.box_rows = rows;
+        a.box_slabs = rows == tile ? hd / 64 : 1;
         const cuuint64_t pages = kv.page_table ? cache_rows / kv.page_rows : 1, per = kv.page_table ? kv.page_rows : cache_rows;
-        const cuuint64_t kd[4] = {hd, p->num_kv_heads, per, pages}, ks[3] = {hd * 2ull, row * 2, pages > 1 ? per * row * 2 : row * 2};
-        const cuuint32_t kb[4] = {64, 1, rows, 1};
-        fine = fine && pr::encode(&m.k, p->dtype, kv.k_base, 4, kd, ks, kb) && pr::encode(&m.v, p->dtype, kv.v_base, 4, kd, ks, kb);
+        // (64 elements, row, slab, kv head, page): a box of several slabs then lies in shared memory slab after slab
+        const cuuint64_t kd[5] = {64, per, hd / 64, p->num_kv_heads, pages}, ks[4] = {row * 2, 128, hd * 2ull, pages > 1 ? per * row * 2 : row * 2};
+        const cuuint32_t kb[5] = {64, rows, a.box_slabs, 1, 1};
+        fine = fine && pr::encode(&m.k, p->dtype, kv.k_base, 5, kd, ks, kb) && pr::encode(&m.v, p->dtype, kv.v_base, 5, kd, ks, kb);
         SHADY_REQUIRE(ctx, fine, SHADY_ERR_CUDA, w + ": cuTensorMapEncodeTiled failed");
     }
     // items: blocks of nt * tpt tokens; a sequence's last block may be partly filled
