@@ -143,7 +143,10 @@ __device__ __forceinline__ void cap_small(uint32_t &s0, uint32_t &s1, float c, f
     asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(p));
     s0 = __float_as_uint(y0); s1 = __float_as_uint(y1);
 }
-// The same for |s c| <= kTanhTiny, where two terms less do.
+// The same for |s c| <= kTanhTiny, where three terms less do (cap 50: 692 us against 788).  A warp chooses by its tile's largest
+// score; where tiles alternate between two forms, fetching their unrolled code costs more than either form alone (cap 35: 837 us,
+// with the longer polynomial only 786).  Staying with the longer form once an item has needed it helps there (784) and
+// costs more at cap 50 (748); a third polynomial in between gains at cap 30 (717 against 780) and loses at 20 (1,123 against 780).
 __device__ __forceinline__ void cap_tiny(uint32_t &s0, uint32_t &s1, float c, float cap2, float add) {
     const unsigned long long x = mul_f32x2(pack_f32x2(__uint_as_float(s0), __uint_as_float(s1)), both(c)), t = mul_f32x2(x, x);
     unsigned long long p = fma2(t, both(kTanhT2 * cap2), both(kTanhT1 * cap2));
