@@ -168,9 +168,10 @@ __device__ __forceinline__ void cap_any(uint32_t &s0, uint32_t &s1, float c, flo
 }
 
 // MODE 0: scale only, 1: tanh cap, 2: distance bias, with or without a cap; 3: tanh cap with a fixed reference.
-// A cap bounds y = z log2(e) by +-cap2, and bf16 weights have the range of f32: with cap2 <= kFixedCap the weights are
-// 2^(y - cap2/2), between 2^(-3/2 cap2) and 2^(cap2/2), and neither a row maximum nor a rescaling of O is needed (4 x 4096
-// batch, cap 50: 700 us, with a running maximum 775).
+// A cap bounds y = z log2(e) by +-cap2, and bf16 weights have the range of f32: with cap2 <= kFixedCap the weights are 2^(y - m)
+// with m the maximum of the row's first tile, or cap2 - 96 where that is larger, so that they lie below 2^96 and what is seen
+// above 2^-126 of the largest.  No running maximum, no rescaling of O (4 x 4096 batch, cap 50: 692 us, with a running
+// maximum 775).  A row that sees one tile, one row at the least, has its largest weight at exactly 1.
 constexpr float kFixedCap = 80.0f;
 template <typename T, int HD, int MODE>
 __global__ void __launch_bounds__(Cfg<HD>::kThreads, 1)
@@ -507,7 +508,6 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const uint32_t t_rel = q * TPT + r / a.G, g = r % a.G;
         const float scale2 = a.rule.scale * kRuleLog2e;
         const float cap_c = a.rule.scale * a.rule.inv_cap, cap2 = a.rule.cap * kRuleLog2e;
-        const float cap_add = MODE == 3 ? -0.5f * cap2 : 0.f;
         bool ok = true;
         uint32_t tc = 0;            // turns taken
         uint32_t cnt = 0, oc = 0;   // score tiles and items of this row tile so far (barrier phases)
@@ -537,7 +537,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
             float slope2 = 0.f;
             if (MODE == 2) slope2 = live ? __ldg(a.rule.slopes + slot[2] * a.G + g) * kRuleLog2e : 0.f;
-            float m_ref = MODE == 3 ? 0.5f * cap2 : -INFINITY, l_sum = 0.f;
+            float m_ref = MODE == 3 ? 0.f : -INFINITY, l_sum = 0.f;   // MODE 3: set by the first tile
             for (uint32_t j = 0; j < n && ok; ++j, k0 = j == turn ? (int32_t)(other * N) : (kRev ? k0 - (int32_t)N : k0 + (int32_t)N)) {
                 const uint32_t b = q * NS + cnt % NS, pb = q * NP + cnt % NP;
                 // the weights' buffer first: the product that read it, kNP tiles back, is done by now, and scores are still to come
@@ -555,6 +555,7 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 mbar_arrive(bar(B_SFREE + b));
                 // ---- the rule: x = z log2(e), or with scale alone the raw product ----
                 if (MODE == 1 || MODE == 3 || (MODE == 2 && a.rule.cap > 0.f)) {
+                    const float cap_add = MODE == 3 ? -m_ref : 0.f;
                     float top[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (uint32_t c = 0; c < N / 32; ++c)
@@ -613,7 +614,21 @@ prefill_rule_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                             if (!(see & (1u << i))) x[c][i] = 0xff800000u;   // -inf
                     }
                 }
-                if constexpr (MODE != 3) {
+                if constexpr (MODE == 3) {
+                    if (j == 0) {
+                        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (uint32_t c = 0; c < N / 32; ++c)
+#pragma unroll
+                            for (uint32_t i = 0; i < 32; i += 2)
+                                mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+                        m_ref = fmaxf(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), cap2 - 96.0f);
+#pragma unroll
+                        for (uint32_t c = 0; c < N / 32; ++c)
+#pragma unroll
+                            for (uint32_t i = 0; i < 32; ++i) x[c][i] = __float_as_uint(__uint_as_float(x[c][i]) - m_ref);
+                    }
+                } else {
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (uint32_t c = 0; c < N / 32; ++c)

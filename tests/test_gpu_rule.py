@@ -637,3 +637,20 @@ def test_launches_wait_for_an_uncollected_timeout(gpu_ctx):
     gpu.synchronize()
     lone.close()
     gpu.close()
+
+
+@pytest.mark.parametrize("rule", [dict(), dict(cap=50.0), dict(cap=55.0), dict(cap=60.0), dict(cap=50.0, slopes=True)])
+@pytest.mark.parametrize("hd,dt", [(128, BF16), (256, BF16), (128, F16)])
+def test_a_query_that_sees_one_row_returns_its_value(gpu_ctx, hd, dt, rule):
+    """The one weight is exactly 1 whatever the score, so the first token of a prompt gets its own V row to the last bit; an
+    approximate reference of the weights would leave a rounding of half a step."""
+    S, nkv, G, t = 9, 2, 4, TORCH_DT[dt]
+    g = torch.Generator().manual_seed(hd)
+    q = (torch.randn(S, nkv * G, hd, generator=g) * 2).to(t).cuda()
+    k, v = (torch.randn(S, nkv, hd, generator=g).to(t).cuda() for _ in range(2))
+    r = ops.ScoreRule(cap=rule.get("cap", 0.0), slopes=torch.full((nkv * G,), 0.3, device="cuda") if rule.get("slopes") else None)
+    out = torch.full_like(q, float("nan"))
+    ops.attn_prefill_rule(gpu_ctx, q=q, cache=ops.KvCacheView(dt, k, v, nkv * hd), cache_rows=S, q_starts=dev_u32(list(range(S + 1))), total_q=S,
+                          kv_lens=dev_u32([1] * S), out=out, head_dim=hd, num_kv_heads=nkv, num_q_heads=nkv * G, num_seqs=S, dtype=dt, rule=r)
+    gpu_ctx.synchronize()
+    assert torch.equal(out, v.repeat_interleave(G, dim=1))
