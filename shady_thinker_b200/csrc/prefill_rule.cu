@@ -10,8 +10,8 @@
 // tensor pipe about 850 clocks (a score MMA with N = 64 takes 70 of them instead of 32: its A tile comes from shared memory
 // at 128 bytes per clock), the exponentials 512, a cap 320 of the FMA pipe; stamps put a tile at about 900 clocks without a
 // rule and 1,100 with a cap, where two warps per scheduler share one FMA pipe and one special function unit.
-// Measured (B200, bf16): 4 x 4096 tokens, 32 heads of 128 over 8, cap 50: 0.70 ms = 785 TFLOP/s, no cap 0.55..0.61 ms =
-// 900..1,010; 8,192 tokens of packed documents behind a window of 2,048: 0.114 ms; 2 x 1024 tokens behind 8,192 rows,
+// Measured (B200, bf16): 4 x 4096 tokens, 32 heads of 128 over 8, cap 50: 0.70..0.73 ms = 750..780 TFLOP/s, no cap 0.55..0.62 ms
+// = 885..1,010; 8,192 tokens of packed documents behind a window of 2,048: 0.114 ms; 2 x 1024 tokens behind 8,192 rows,
 // head_dim 256, distance bias: 0.143 ms = 1,030 TFLOP/s; seven prompts of up to 301 tokens, f16, capped: 15.4 us.
 //
 //   * The query heads of a kv head share a row tile: row r of a tile is token r / G, head r % G (G heads per kv head,
@@ -143,7 +143,7 @@ __device__ __forceinline__ void cap_small(uint32_t &s0, uint32_t &s1, float c, f
     asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(p));
     s0 = __float_as_uint(y0); s1 = __float_as_uint(y1);
 }
-// The same for |s c| <= kTanhTiny, where three terms less do (cap 50: 692 us against 788).  A warp chooses by its tile's largest
+// The same for |s c| <= kTanhTiny, where three terms less do (cap 50: 740 us against 788 when it was added).  A warp chooses by its tile's largest
 // score; where tiles alternate between two forms, fetching their unrolled code costs more than either form alone (cap 35: 837 us,
 // with the longer polynomial only 786).  Staying with the longer form once an item has needed it helps there (784) and
 // costs more at cap 50 (748); a third polynomial in between gains at cap 30 (717 against 780) and loses at 20 (1,123 against 780).
@@ -170,7 +170,7 @@ __device__ __forceinline__ void cap_any(uint32_t &s0, uint32_t &s1, float c, flo
 // MODE 0: scale only, 1: tanh cap, 2: distance bias, with or without a cap; 3: tanh cap with a fixed reference.
 // A cap bounds y = z log2(e) by +-cap2, and bf16 weights have the range of f32: with cap2 <= kFixedCap the weights are 2^(y - m)
 // with m the maximum of the row's first tile, or cap2 - 96 where that is larger, so that they lie below 2^96 and what is seen
-// above 2^-126 of the largest.  No running maximum, no rescaling of O (4 x 4096 batch, cap 50: 692 us, with a running
+// above 2^-126 of the largest.  No running maximum, no rescaling of O (4 x 4096 batch, cap 50: 714 us, with a running
 // maximum 775).  A row that sees one tile, one row at the least, has its largest weight at exactly 1.
 constexpr float kFixedCap = 80.0f;
 template <typename T, int HD, int MODE>
